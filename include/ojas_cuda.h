@@ -193,6 +193,57 @@ ojc_status ojc_kv_cache_write(ojc_backend* be, ojc_tensor* cache, const ojc_tens
 ojc_status ojc_cached_attention_forward(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_cache, const ojc_tensor* v_cache, uint64_t kv_len, int64_t window,
                                         ojc_tensor* out);
 
+/* ---- decode over a paged KV cache (no counterpart in the reference, whose cache is one ring per sequence): requests of different lengths share
+ *      a pool of pages [P, page, Hkv, D]; row b of block_tables [B, W] names the pages of request b in order, so position p of request b is slot
+ *      block_tables[b][p / page] * page + p % page of the pool. The new tokens of all requests lie behind one another in [N, ...] tensors, request b's
+ *      in rows starts[b] .. starts[b + 1) - 1, and its token i takes the cache place cached_lens[b] + i. New tokens are a piece of a prompt, one decoded
+ *      token, or a tree of drafts whose places are consecutive but whose positions (for rotation and windows) go by depth. A pass over a layer is
+ *      paged_plan (once), rope_forward on q, paged_kv_write of k and v, paged_attention_forward; nothing in it is read back to the host, and shapes
+ *      depend on capacities alone, so a pass may be captured from ojc_stream into a graph (replay it on that stream; give paged_attention_forward a
+ *      workspace of the caller's). All index tensors are U32; OJC_NONE stands for "no slot" and "no parent". What the host cannot see is checked on
+ *      the device: a page, slot, length or parent out of range is skipped and surfaces as OutOfRange at the next sync. */
+#define OJC_NONE 0xffffffffu
+/* Block tables and slot maps from lengths. cached_lens, new_lens [B]; parents [N] (optional): draft i's parent as its index among the request's
+ * own drafts, below i, or OJC_NONE for a child of the last cached token; without parents each token follows the one before it. New pages are taken from
+ * free_pages [F] from entry *free_head on, requests in order, and entered in block_tables (its other entries stay as they are); *free_head_out, another
+ * tensor, is the first entry left. Written: starts [B + 1], slots [N], positions [N] (cached length + depth), and masks [N, words] (optional): bit j of
+ * row i says that token j of the request is i or an ancestor of i. Rows behind the last token, and tokens without a page, get slot OJC_NONE; the former
+ * position 0 and no mask bits. Too few free pages: CapacityExceeded at the next sync. B up to 24,000. */
+ojc_status ojc_paged_plan(ojc_backend* be, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* parents, const ojc_tensor* free_pages, const ojc_tensor* free_head,
+                          int64_t page_size, ojc_tensor* block_tables, ojc_tensor* starts, ojc_tensor* slots, ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out);
+/* Rotary positions without tables: the leading rotary_dim elements of each head are pairs, (i, i + rotary_dim / 2) in the half layout or
+ * (2i, 2i + 1) in the interleaved one, and pair i is turned by position * f_i radians and scaled by amplitude; the rest passes through.
+ * f_i = base^(-2i / rotary_dim), stretched for contexts beyond original_length: linear f_i / factor; base: base * factor^(R / (R - 2)) for base;
+ * by turns: with t_i = original_length * f_i / 2 pi and w = clamp((t_i - low_turns) / (high_turns - low_turns), 0, 1), f_i * (w + (1 - w) / factor).
+ * ojc_rope_plan (host only) forms the frequencies in extended precision as 64-bit fractions of a turn, so that far positions lose nothing. */
+#define OJC_ROPE_MAX_PAIRS 128
+typedef struct ojc_rope_spec {
+  int32_t rotary_dim, layout /* 0 half, 1 interleaved */, scaling /* 0 none, 1 linear, 2 base, 3 by turns */;
+  double base, factor, original_length, low_turns, high_turns, amplitude;
+} ojc_rope_spec;
+typedef struct ojc_rope { int32_t rotary_dim, layout; float amplitude; uint32_t reserved; uint64_t turns[OJC_ROPE_MAX_PAIRS]; } ojc_rope;
+ojc_status ojc_rope_plan(const ojc_rope_spec* spec, ojc_rope* rope);
+/* x, y [N, H, D] or [B, T, H, D], F32 or BF16, read and written through their strides (D contiguous); y may be x itself. positions [N], or for rank 4
+ * [B * T] or [T] for every batch row. The backward is the opposite turn with the same amplitude. */
+ojc_status ojc_rope_forward(ojc_backend* be, const ojc_rope* rope, const ojc_tensor* x, const ojc_tensor* positions, ojc_tensor* y);
+ojc_status ojc_rope_backward(ojc_backend* be, const ojc_rope* rope, const ojc_tensor* grad_y, const ojc_tensor* positions, ojc_tensor* grad_x);
+/* k, v [N, Hkv, D] (F32 or BF16) into the slots of k_pages, v_pages [P, page, Hkv, D] (F32 or BF16, rounded once), all through their strides (D
+ * contiguous). With rope (and positions [N]) k is rotated on the way. A row with slot OJC_NONE is skipped; the other slots of a call are distinct. */
+ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* v_pages, const ojc_tensor* k, const ojc_tensor* v, const ojc_tensor* slots, const ojc_rope* rope,
+                              const ojc_tensor* positions);
+/* q, out [N, H, D] against the pages (all F32, or all BF16 with f32 sums), through their strides (D contiguous, at most 256); lse [N, H] F32 (optional).
+ * Head h reads KV head h / (H / Hkv), the scale is 1 / sqrt(D). Token i of request b sees the cached places below cached_lens[b] and, of the
+ * request's new tokens, those whose bits are set in row i of masks [N, words], or without masks those up to itself; of all these, with window >= 1,
+ * only those whose position is above its own minus window (the position of a cached place is the place, that of a new token its entry of positions
+ * [N]; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). Masked places are never
+ * looked at: NaN or infinity there does no harm. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
+ * non-finite value that a row does see surfaces as NonFinite. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
+ * NULL for the library's own (refused while the stream is being captured). */
+ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, uint64_t* bytes);
+ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, const ojc_tensor* v_pages, const ojc_tensor* block_tables, const ojc_tensor* cached_lens,
+                                       const ojc_tensor* starts, const ojc_tensor* masks, const ojc_tensor* positions, int64_t window, ojc_tensor* out, ojc_tensor* lse, void* workspace,
+                                       uint64_t workspace_bytes);
+
 /* ---- gradient plumbing and optimizers */
 ojc_status ojc_accumulate_grad(ojc_backend* be, ojc_tensor* acc, const ojc_tensor* grad);                                    /* :1483 acc += grad */
 ojc_status ojc_scale_grad(ojc_backend* be, ojc_tensor* grad, float scale);                                                   /* :1502 */

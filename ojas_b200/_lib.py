@@ -41,6 +41,15 @@ class StepReport(C.Structure):
     _fields_ = [("loss", C.c_float), ("grad_norm", C.c_float), ("step", C.c_uint64), ("tokens", C.c_uint64), ("lr_multiplier", C.c_double)]
 
 
+class RopeSpec(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rotary_dim", "layout", "scaling")] + [(n, C.c_double) for n in (
+        "base", "factor", "original_length", "low_turns", "high_turns", "amplitude")]
+
+
+class Rope(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("layout", C.c_int32), ("amplitude", C.c_float), ("reserved", C.c_uint32), ("turns", C.c_uint64 * 128)]
+
+
 def load() -> C.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(f"{LIB_PATH} is missing: build it with `make -C {_PKG / 'csrc'}` (or __graft_entry__.build()); "

@@ -127,6 +127,36 @@ class MuonNs5Config:
         return _lib.MuonConfig(self.lr, self.momentum, self.weight_decay, int(self.nesterov), int(self.ns5_bf16))
 
 
+@dataclass
+class RopeSpec:
+    """Rotary positions of a head's leading `rotary_dim` elements (ojc_rope_spec). layout: "half" pairs (i, i + rotary_dim / 2), "interleaved" (2i, 2i + 1).
+    scaling stretches the context by `factor`: "linear" divides every frequency, "base" raises the base, "by_turns" divides only those of pairs that turn
+    fewer than `low_turns` times within `original_length`, keeps those above `high_turns` and blends between. `amplitude` scales the rotated part."""
+    rotary_dim: int
+    base: float = 10000.0
+    layout: str = "half"
+    scaling: str = "none"
+    factor: float = 1.0
+    original_length: float = 0.0
+    low_turns: float = 1.0
+    high_turns: float = 32.0
+    amplitude: float = 1.0
+
+    def c(self):
+        return _lib.RopeSpec(self.rotary_dim, {"half": 0, "interleaved": 1}[self.layout], {"none": 0, "linear": 1, "base": 2, "by_turns": 3}[self.scaling],
+                             self.base, self.factor, self.original_length, self.low_turns, self.high_turns, self.amplitude)
+
+
+@dataclass
+class PagedPlan:
+    """What ojc_paged_plan writes (besides the block tables): see CudaBackend.paged_plan."""
+    starts: Tensor
+    slots: Tensor
+    positions: Tensor
+    masks: Tensor | None
+    free_head: Tensor
+
+
 class CudaBackend:
     """`impl Backend for CudaBackend` on B200. Opening refuses anything but an sm_100 device; there is no host path."""
 
@@ -439,6 +469,67 @@ class CudaBackend:
         out = self.empty(q.shape, DType.F32)
         _check(lib.ojc_cached_attention_forward(self._handle, _p(q), _p(k_cache), _p(v_cache), C.c_uint64(kv_len), C.c_int64(-1 if window is None else window), _p(out)))
         return out
+
+    # ---- decode over a paged KV cache
+    def paged_plan(self, cached_lens: Tensor, new_lens: Tensor, free_pages: Tensor, free_head: Tensor, block_tables: Tensor, page_size: int, tokens: int | None = None,
+                   parents: Tensor | None = None, mask_words: int = 0, starts: Tensor | None = None, slots: Tensor | None = None, positions: Tensor | None = None,
+                   masks: Tensor | None = None, free_head_out: Tensor | None = None) -> PagedPlan:
+        """Plan of a pass over a paged cache (ojc_paged_plan): new tokens `new_lens` [B] behind `cached_lens` [B] get pages from `free_pages` (entered in
+        `block_tables` [B, W]), slots and positions, and for trees of drafts ancestor masks of `mask_words` words. `tokens` is the capacity N of the
+        outputs that are not given (by default that of `parents`); rows behind the last token get slot 0xffffffff."""
+        if slots is None and tokens is None:
+            if parents is None:
+                raise OjasError(STATUS_NAMES.index("Shape"), "paged_plan: give the capacity `tokens`, `parents` or `slots`")
+            tokens = parents.shape[0]
+        n = slots.shape[0] if slots is not None else tokens
+        starts = starts if starts is not None else self.empty((cached_lens.shape[0] + 1,), DType.U32)
+        slots = slots if slots is not None else self.empty((n,), DType.U32)
+        positions = positions if positions is not None else self.empty((n,), DType.U32)
+        if masks is None and mask_words:
+            masks = self.empty((n, mask_words), DType.U32)
+        free_head_out = free_head_out if free_head_out is not None else self.empty((1,), DType.U32)
+        _check(lib.ojc_paged_plan(self._handle, _p(cached_lens), _p(new_lens), _p(parents), _p(free_pages), _p(free_head), C.c_int64(page_size), _p(block_tables), _p(starts),
+                                  _p(slots), _p(positions), _p(masks), _p(free_head_out)))
+        return PagedPlan(starts, slots, positions, masks, free_head_out)
+
+    @staticmethod
+    def rope_plan(spec: RopeSpec) -> "_lib.Rope":
+        """The frequencies of `spec` as the rotary entry points take them; keep it for as many calls as use it (host arithmetic only)."""
+        rope, cs = _lib.Rope(), spec.c()
+        _check(lib.ojc_rope_plan(C.byref(cs), C.byref(rope)))
+        return rope
+
+    def rope_forward(self, x: Tensor, positions: Tensor, rope: "_lib.Rope", out: Tensor | None = None) -> Tensor:
+        """x [N, H, D] or [B, T, H, D] (any strides, D contiguous) rotated by positions [N] (or [B * T], or [T]); `out` may be x itself."""
+        out = out if out is not None else self.empty(x.shape, x.dtype)
+        _check(lib.ojc_rope_forward(self._handle, C.byref(rope), _p(x), _p(positions), _p(out)))
+        return out
+
+    def rope_backward(self, grad_y: Tensor, positions: Tensor, rope: "_lib.Rope", out: Tensor | None = None) -> Tensor:
+        out = out if out is not None else self.empty(grad_y.shape, grad_y.dtype)
+        _check(lib.ojc_rope_backward(self._handle, C.byref(rope), _p(grad_y), _p(positions), _p(out)))
+        return out
+
+    def paged_kv_write(self, k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, slots: Tensor, rope: "_lib.Rope | None" = None, positions: Tensor | None = None):
+        """k, v [N, Hkv, D] into the slots of the pages [P, page, Hkv, D]; with `rope` and `positions` k is rotated on the way."""
+        _check(lib.ojc_paged_kv_write(self._handle, _p(k_pages), _p(v_pages), _p(k), _p(v), _p(slots), C.byref(rope) if rope is not None else None, _p(positions)))
+
+    def paged_attention_workspace(self, q: Tensor, k_pages: Tensor) -> Tensor:
+        """A workspace for paged_attention_forward on these shapes (of which one pass at a time makes use)."""
+        need = C.c_uint64()
+        _check(lib.ojc_paged_attention_workspace_bytes(self._handle, _p(q), _p(k_pages), C.byref(need)))
+        return self.empty(((need.value + 3) // 4,), DType.F32)
+
+    def paged_attention_forward(self, q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, cached_lens: Tensor, starts: Tensor, masks: Tensor | None = None,
+                                positions: Tensor | None = None, window: int | None = None, out: Tensor | None = None, lse: Tensor | None = None, workspace: Tensor | None = None):
+        """(out [N, H, D], lse [N, H]) of the new tokens' queries over the cached places of their requests and, by `masks` or causally, over the new
+        tokens themselves (ojc_paged_attention_forward)."""
+        out = out if out is not None else self.empty(q.shape, q.dtype)
+        lse = lse if lse is not None else self.empty(q.shape[:2], DType.F32)
+        _check(lib.ojc_paged_attention_forward(self._handle, _p(q), _p(k_pages), _p(v_pages), _p(block_tables), _p(cached_lens), _p(starts), _p(masks), _p(positions),
+                                               self._window(window), _p(out), _p(lse), C.c_void_p(workspace.ptr if workspace is not None else None),
+                                               C.c_uint64(workspace.numel * workspace.dtype.size if workspace is not None else 0)))
+        return out, lse
 
     # ---- in-place gradient plumbing and optimizers
     def accumulate_grad(self, acc: Tensor, grad: Tensor):

@@ -33,6 +33,9 @@ enum OjcOp : uint32_t {
   OP_ADD, OP_LINEAR_CE, OP_CE, OP_ACCUMULATE, OP_SCALE, OP_CLIP, OP_ADAMW, OP_MUON, OP_ARGMAX, OP_CAST, OP_GEMM_WAIT,
   OP_CACHED_ATTN, OP_TOPK,
   OP_ID_RANGE,  // a token id or target outside the vocabulary: reported as OutOfRange
+  OP_PAGED_ATTN,
+  OP_PAGED_RANGE,  // a page, slot, length or tree parent outside its table: reported as OutOfRange
+  OP_PAGED_FULL,   // the free pages ran out: reported as CapacityExceeded
   OP_COUNT
 };
 const char* ojc_op_name(uint32_t op);

@@ -1,0 +1,34 @@
+// Shared by the kernels over a paged KV cache: the pages' view, the pass's index tables and the rotation of a pair.
+#pragma once
+#include "common.cuh"
+
+// [P, page, Hkv, D] through strides in elements; D contiguous
+template <class P>
+struct PagesView {
+  P* ptr;
+  int64_t sp, st, sh;   // page, place in the page, head
+};
+template <class P>
+inline PagesView<P> pages_view(const ojc_tensor* t) { return PagesView<P>{(P*)t->data, t->stride[0], t->stride[1], t->stride[2]}; }
+
+// [N, H, D] through strides; D contiguous
+template <class P>
+struct RowsView {
+  P* ptr;
+  int64_t sn, sh;
+};
+template <class P>
+inline RowsView<P> rows_view(const ojc_tensor* t) { return RowsView<P>{(P*)t->data, t->stride[0], t->stride[1]}; }
+
+#ifdef __CUDACC__
+// Rotation of a pair: the angle is position x frequency with the frequency in 2^-64 turns, so the product modulo 2^64 IS the angle's fraction of a
+// turn, exact to position x 2^-64 however far the position; its upper half as a signed integer is the angle / pi in [-1, 1) x 2^31.
+__device__ __forceinline__ void rope_turn(uint64_t turns, uint32_t position, float amplitude, float* c, float* s) {
+  const uint64_t t = turns * position;
+  sincospif((float)(int32_t)(uint32_t)(t >> 32) * 4.656612873077393e-10f, s, c);
+  *c *= amplitude;
+  *s *= amplitude;
+}
+#endif
+
+ojc_status rope_check(const char* op, const ojc_rope* rope, int64_t head_dim);

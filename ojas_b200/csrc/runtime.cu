@@ -19,7 +19,7 @@ static const char* kOpNames[OP_COUNT] = {"none", "embedding", "linear", "rms_nor
                                          "linear_cross_entropy_mean", "cross_entropy_mean", "accumulate_grad",
                                          "scale_grad", "clip_grad_norm", "adamw_step", "muon_ns5_step", "argmax_rows",
                                          "cast", "gemm_pipeline_wait", "cached_attention_forward", "topk_rows",
-                                         "token id or target"};
+                                         "token id or target", "paged_attention_forward", "paged cache", "paged_plan"};
 const char* ojc_op_name(uint32_t op) { return op < OP_COUNT ? kOpNames[op] : "unknown"; }
 
 ojc_status ojc_fail(ojc_status st, const char* op, const std::string& detail) {
@@ -228,6 +228,8 @@ static ojc_status report_fault(ojc_backend* be, const char* op) {
   be->fault_host[0] = be->fault_host[1] = 0;
   cudaMemsetAsync(be->fault_dev, 0, 8, be->stream);
   if (first == OP_ID_RANGE) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "a token id or target on the device is outside the vocabulary");
+  if (first == OP_PAGED_RANGE) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "a page, slot, length or tree parent of the paged cache on the device is out of range");
+  if (first == OP_PAGED_FULL) return ojc_fail(OJC_ERR_CAPACITY_EXCEEDED, op, "the free pages of the paged cache ran out on the device");
   if (first == OP_GEMM_WAIT) return ojc_fail(OJC_ERR_WAIT_TIMEOUT, op, "a tensor-pipeline wait inside a GEMM kernel ran out");
   return ojc_fail(OJC_ERR_NON_FINITE, ojc_op_name(first), std::string("non-finite value raised on the device, reported at ") + op);
 }

@@ -1,0 +1,508 @@
+"""The paged-cache operators against their 64-bit definitions (paged_reference.py), at the sizes, masks and layouts where they can go wrong."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+NONE = ref.NONE
+HALF_BF16, HALF_F32 = 2.0 ** -8, 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def be():
+    from ojas_b200 import CudaBackend
+    backend = CudaBackend(0, 32 << 30)
+    yield backend
+    backend.sync()
+    backend.close()
+
+
+def u32(be, a):
+    return be.upload(np.ascontiguousarray(a).astype(np.int64).astype(np.uint32))
+
+
+def floats(be, a, bf16):
+    from ojas_b200 import DType
+    return be.upload(np.ascontiguousarray(a, np.float32), DType.BF16 if bf16 else None)
+
+
+def strided(be, a, bf16, pad, order=None):
+    """A view of `a` whose storage has its axes in `order` and rows of `pad` more elements than the last axis."""
+    from ojas_b200 import Tensor
+    order = list(order or range(a.ndim))
+    wide = np.full([a.shape[d] for d in order[:-1]] + [a.shape[order[-1]] + pad], 7.0, np.float32)
+    wide[..., : a.shape[order[-1]]] = a.transpose(order)
+    base = floats(be, wide, bf16)
+    strides = [0] * a.ndim
+    for d, s in zip(order, base.strides):
+        strides[d] = s
+    return Tensor(be, base.ptr, a.shape, base.dtype, strides, owner=base), base
+
+
+# ---------------------------------------------------------------------------------------------------------------- plan
+
+def tree_parents(rng, new, spread=3):
+    """Per token the parent's index among the request's drafts; some roots in the middle, the first one always a root."""
+    out = []
+    for n in new:
+        for i in range(n):
+            p = i - 1 - int(rng.integers(0, spread))
+            out.append(p if p >= 0 else NONE)
+    return np.array(out, np.int64)
+
+
+@pytest.mark.parametrize("cached,new,page,tree,pad", [
+    ([0], [1], 1, False, 0), ([5], [1], 16, False, 3), ([16], [16], 16, True, 0), ([15, 16, 17, 0], [1, 1, 1, 33], 16, True, 5),
+    ([0, 0, 0], [0, 0, 7], 4, True, 1), ([3, 9, 1], [4, 0, 0], 8, False, 2), ([100, 7, 31], [40, 64, 5], 20, True, 0), ([4095] * 5, [300, 1, 77, 130, 2], 64, False, 9),
+    (list(range(300)), [i % 5 for i in range(300)], 7, True, 4), ([11] * 1000, [3] * 1000, 32, False, 0)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_plan(be, cached, new, page, tree, pad, masked):
+    rng = np.random.default_rng(len(cached) + page)
+    n, words = sum(new), (max(new) + 31) // 32 if masked else 0
+    held, total = [-(-c // page) for c in cached], [-(-(c + k) // page) for c, k in zip(cached, new)]
+    pool = rng.permutation(sum(total) + 11)
+    tables = np.full((len(cached), max(total) + 2), 0xABCD, np.int64)
+    at = 0
+    for b, k in enumerate(held):
+        tables[b, :k] = pool[at:at + k]
+        at += k
+    free, head = np.concatenate([[0xDEAD] * 2, pool[at:]]), 2
+    parents = np.concatenate([tree_parents(rng, new), np.zeros(pad, np.int64)]) if tree else None
+    want = ref.plan(cached, new, free, head, tables, page, n + pad, parents, words)
+    dt, dh = u32(be, tables), u32(be, [head])
+    for again in range(2):                       # the same lengths once more: the same pages, nothing moves
+        got = be.paged_plan(u32(be, cached), u32(be, new), u32(be, free), dh, dt, page, tokens=n + pad, parents=u32(be, parents) if tree else None, mask_words=words)
+        assert np.array_equal(got.starts.numpy(), want[0]) and np.array_equal(got.slots.numpy(), want[1]) and np.array_equal(got.positions.numpy(), want[2])
+        if words:
+            assert np.array_equal(got.masks.numpy(), want[3])
+        assert got.free_head.numpy()[0] == want[4] and np.array_equal(dt.numpy(), want[5]) and dh.numpy()[0] == head
+
+
+def test_plan_with_the_largest_batch(be):
+    batch = 24000
+    cached, new = np.arange(batch) % 37, (np.arange(batch) * 7) % 3
+    free = np.arange(batch * 2)[::-1].copy()
+    tables = np.zeros((batch, 8), np.int64)
+    want = ref.plan(cached, new, free, 1, tables, 16, int(new.sum()))
+    dt = u32(be, tables)
+    got = be.paged_plan(u32(be, cached), u32(be, new), u32(be, free), u32(be, [1]), dt, 16, tokens=int(new.sum()))
+    assert np.array_equal(got.slots.numpy(), want[1]) and np.array_equal(got.starts.numpy(), want[0]) and np.array_equal(dt.numpy(), want[5])
+
+
+@pytest.mark.parametrize("what,kind", [("free", "CapacityExceeded"), ("width", "OutOfRange"), ("tokens", "OutOfRange"), ("parent", "OutOfRange"), ("words", "OutOfRange"),
+                                       ("entry", "OutOfRange"), ("head", "CapacityExceeded"), ("length", "OutOfRange")])
+def test_plan_reports_what_only_the_device_sees(be, what, kind):
+    from ojas_b200 import OjasError
+    cached, new, page = [30, 8], [5, 40], 8
+    free, head, width, tokens, words = np.arange(20) + 50, 0, 8, 45, 2
+    tables = np.arange(2 * width).reshape(2, width)
+    parents = tree_parents(np.random.default_rng(0), new)
+    if what == "free":
+        free = free[:3]
+    if what == "width":
+        tables = tables[:, :5]
+    if what == "tokens":
+        tokens, parents = 44, parents[:44]
+    if what == "parent":
+        parents[9] = 4
+    if what == "words":
+        words = 1
+    if what == "entry":
+        tables[0, 3] = NONE
+    if what == "head":
+        head = 25
+    if what == "length":
+        cached = [30, NONE - 3]
+    dt = u32(be, tables)
+    got = be.paged_plan(u32(be, cached), u32(be, new), u32(be, free), u32(be, [head]), dt, page, tokens=tokens, parents=u32(be, parents), mask_words=words)
+    with pytest.raises(OjasError) as e:
+        be.sync()
+    assert e.value.kind == kind
+    slots = got.slots.numpy()                    # reported once; slots that could be formed are slots of known pages
+    known = set(int(p) for p in free) | set(int(p) for p in tables.ravel())
+    assert all(int(s) // page in known for s in slots if s != NONE)
+    if what == "free":
+        assert np.sum(slots == NONE) > 0 and got.free_head.numpy()[0] == 3
+
+
+# ---------------------------------------------------------------------------------------------------------------- rope
+
+ROPE = [(1, 1, 2, 2), (5, 3, 64, 64), (7, 12, 64, 32), (130, 2, 80, 20), (33, 5, 96, 96), (9, 4, 128, 128), (3, 2, 256, 256), (17, 1, 66, 34), (65, 40, 128, 64), (2, 3, 200, 8),
+        (1000, 8, 64, 64)]
+
+
+def rope_bound(x, freqs, amplitude, half_out):
+    """A turned pair: the angle is off by at most 2^-24 of pi where it is rounded and 2^-22 in its sine and cosine; two products and a sum of 2^-24 each."""
+    size = np.abs(amplitude) * np.sqrt(2.0) * np.abs(x).max()
+    return (half_out + 2.0 ** -20) * size
+
+
+@pytest.mark.parametrize("n,h,d,rotary", ROPE)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rope_forward_and_backward(be, n, h, d, rotary, layout, bf16):
+    from ojas_b200 import RopeSpec
+    rng = np.random.default_rng(n + d)
+    x = rng.standard_normal((n, h, d)).astype(np.float32)
+    x = ref.round_bf16(x) if bf16 else x
+    positions = rng.integers(0, 1 << 20, n)
+    positions[0] = NONE if n % 2 else 0                 # as far as a position goes
+    spec = RopeSpec(rotary, layout=layout, scaling="by_turns", factor=8.0, original_length=4096.0, amplitude=1.2)
+    f = ref.frequencies(rotary, scaling="by_turns", factor=8.0, original=4096.0)
+    # the reference's own angles: numpy's frequencies are good to 2^-50 or so, times the position
+    angle_error = positions.max() * 2.0 ** -50
+    half = HALF_BF16 if bf16 else HALF_F32
+    plan = be.rope_plan(spec)
+    for fn, back in ((be.rope_forward, False), (be.rope_backward, True)):
+        got = fn(floats(be, x, bf16), u32(be, positions), plan).numpy()
+        want = ref.rotate(x, positions, f, layout, 1.2, back)
+        assert np.all(np.abs(got - want) <= rope_bound(x, f, 1.2, half) + angle_error * np.abs(x).max())
+        assert np.array_equal(got[..., rotary:], x[..., rotary:])
+    xs, base = strided(be, x, bf16, 6)
+    inplace = be.rope_forward(xs, u32(be, positions), plan, out=xs)
+    assert inplace is xs
+    whole = base.numpy()
+    assert np.array_equal(whole[..., :d], be.rope_forward(floats(be, x, bf16), u32(be, positions), plan).numpy()) and np.all(whole[..., d:] == 7.0)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rope_rank_4_broadcasts_positions_and_reads_permuted_views(be, bf16):
+    from ojas_b200 import RopeSpec
+    rng = np.random.default_rng(2)
+    b, time, h, d = 3, 17, 4, 64
+    x = ref.round_bf16(rng.standard_normal((b, time, h, d)))
+    positions = rng.integers(0, 5000, time)
+    plan = be.rope_plan(RopeSpec(d))
+    flat = be.rope_forward(floats(be, x.reshape(b * time, h, d), bf16), u32(be, np.tile(positions, b)), plan).numpy().reshape(x.shape)
+    assert np.array_equal(be.rope_forward(floats(be, x, bf16), u32(be, positions), plan).numpy(), flat)
+    assert np.array_equal(be.rope_forward(floats(be, x, bf16), u32(be, np.tile(positions, (b, 1))), plan).numpy(), flat)
+    heads_first = floats(be, x.transpose(0, 2, 1, 3), bf16).permuted((0, 2, 1, 3))        # [B, H, T, D] storage
+    assert np.array_equal(be.rope_forward(heads_first, u32(be, positions), plan).numpy(), flat)
+
+
+def test_rope_agrees_with_the_table_form(be):
+    """rope_half_split_forward on tables of the same angles."""
+    from ojas_b200 import RopeSpec
+    rng = np.random.default_rng(3)
+    b, time, h, d = 2, 50, 3, 64
+    x = rng.standard_normal((b, time, h, d)).astype(np.float32)
+    angle = np.arange(time)[:, None] * ref.frequencies(d)[None]
+    cos, sin = np.cos(np.concatenate([angle, angle], 1)).astype(np.float32), np.sin(np.concatenate([angle, angle], 1)).astype(np.float32)
+    got = be.rope_forward(be.upload(x), u32(be, np.arange(time)), be.rope_plan(RopeSpec(d))).numpy()
+    want = be.rope_half_split_forward(be.upload(x), be.upload(cos), be.upload(sin)).numpy()
+    assert np.abs(got - want).max() <= 2 * rope_bound(x, None, 1.0, HALF_F32)
+
+
+def test_rope_gradient_is_that_of_the_forward(be):
+    """Differences of <g, rope(x)>: the map is linear, so <g, rope(x + e) - rope(x)> = <rope_backward(g), e> up to f32 rounding."""
+    from ojas_b200 import RopeSpec
+    rng = np.random.default_rng(4)
+    x, g, e = (rng.standard_normal((21, 3, 32)).astype(np.float32) for _ in range(3))
+    positions, plan = u32(be, rng.integers(0, 100000, 21)), be.rope_plan(RopeSpec(24, layout="interleaved", scaling="linear", factor=3.0, amplitude=0.7))
+    gx = be.rope_backward(be.upload(g), positions, plan).numpy().astype(np.float64)
+    d = be.rope_forward(be.upload(x + e), positions, plan).numpy().astype(np.float64) - be.rope_forward(be.upload(x), positions, plan).numpy()
+    left, right = (g.astype(np.float64) * d).sum(), (gx * e).sum()
+    assert abs(left - right) <= 2.0 ** -20 * np.abs(g).astype(np.float64).ravel() @ (np.abs(d) + np.abs(x) + np.abs(e)).ravel()
+
+
+# ---------------------------------------------------------------------------------------------------------------- write
+
+@pytest.mark.parametrize("n,h,d,page,rotary,layout", [(1, 1, 8, 1, 0, "half"), (5, 2, 64, 16, 64, "half"), (67, 3, 128, 16, 64, "interleaved"), (9, 8, 80, 20, 80, "half"),
+                                                      (130, 1, 66, 7, 34, "half"), (33, 12, 64, 64, 0, "half"), (300, 4, 128, 32, 128, "half")])
+@pytest.mark.parametrize("src,dst", [(False, False), (False, True), (True, True), (True, False)])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_write(be, n, h, d, page, rotary, layout, src, dst, heads_first):
+    from ojas_b200 import RopeSpec
+    rng = np.random.default_rng(n + d)
+    pages = -(-n // page) + 3
+    k, v = (rng.standard_normal((n, h, d)).astype(np.float32) for _ in range(2))
+    if src:
+        k, v = ref.round_bf16(k), ref.round_bf16(v)
+    slots = rng.permutation(pages * page)[:n]
+    slots[n // 2] = NONE if n > 2 else slots[n // 2]
+    positions = rng.integers(0, 1 << 20, n)
+    old = ref.round_bf16(rng.standard_normal((2, pages, page, h, d)))
+    order = (0, 2, 1, 3) if heads_first else None
+    (kp, k_base), (vp, v_base) = strided(be, old[0], dst, 8 if heads_first else 0, order), strided(be, old[1], dst, 8 if heads_first else 0, order)
+    fused, _ = strided(be, np.concatenate([k, v], 1), src, 0)
+    from ojas_b200 import Tensor
+    dk = Tensor(be, fused.ptr, k.shape, fused.dtype, fused.strides, owner=fused)
+    dv = Tensor(be, fused.ptr + h * d * fused.dtype.size, v.shape, fused.dtype, fused.strides, owner=fused)
+    be.paged_kv_write(kp, vp, dk, dv, u32(be, slots), rope=be.rope_plan(RopeSpec(rotary, layout=layout)) if rotary else None, positions=u32(be, positions) if rotary else None)
+    live = slots != NONE
+    want_k = ref.rotate(k, positions, ref.frequencies(rotary), layout) if rotary else k.astype(np.float64)
+    half = HALF_BF16 if dst else HALF_F32
+    for base, fill, rows, tol in ((k_base, old[0], want_k, rope_bound(k, None, 1.0, half) + 2.0 ** -30 if rotary else 0.0), (v_base, old[1], v, 0.0)):
+        got = base.numpy()[..., :d]
+        got = (got.transpose(0, 2, 1, 3) if heads_first else got).reshape(pages * page, h, d)
+        untouched = np.setdiff1d(np.arange(pages * page), slots[live])
+        assert np.array_equal(got[untouched], fill.reshape(-1, h, d)[untouched])
+        want = rows[live]
+        if tol == 0.0:
+            assert np.array_equal(got[slots[live]], ref.round_bf16(want) if dst else want.astype(np.float32))
+        else:
+            assert np.all(np.abs(got[slots[live]] - want) <= tol)
+
+
+def test_write_skips_and_reports_slots_outside_the_pages(be):
+    from ojas_b200 import OjasError
+    kp, vp = be.zeros((2, 4, 1, 8)), be.zeros((2, 4, 1, 8))
+    k = be.upload(np.ones((3, 1, 8), np.float32))
+    be.paged_kv_write(kp, vp, k, k, u32(be, [7, 8, NONE]))
+    with pytest.raises(OjasError) as e:
+        be.sync()
+    assert e.value.kind == "OutOfRange"
+    want = np.zeros((8, 8)); want[7] = 1
+    assert np.array_equal(kp.numpy().reshape(8, 8), want) and np.array_equal(vp.numpy().reshape(8, 8), want)
+
+
+# ---------------------------------------------------------------------------------------------------------------- attention
+
+class Case:
+    """Requests over a shuffled pool whose unused places hold NaN; trees of drafts unless `tree` is False."""
+
+    def __init__(self, seed, cached, new, h, hk, d, page, tree=True, bf16=True, words_more=0, pad=0, scale=1.0):
+        rng = np.random.default_rng(seed)
+        self.rng, self.bf16, self.page = rng, bf16, page
+        self.cached, self.new = np.array(cached), np.array(new)
+        self.starts = np.concatenate([[0], np.cumsum(new)])
+        n, total = int(sum(new)), -(-(self.cached + self.new) // page)
+        pool = int(total.sum()) + 3
+        order, self.tables, at = rng.permutation(pool), np.full((len(cached), int(total.max()) + 1), 0x7FFFFFFF, np.int64), 0
+        self.k = np.full((pool, page, hk, d), np.nan, np.float32)
+        self.v = np.full((pool, page, hk, d), np.nan, np.float32)
+        for b, k in enumerate(total):
+            self.tables[b, :k] = order[at:at + k]
+            at += k
+            p = np.arange(self.cached[b] + self.new[b])
+            for pages in (self.k, self.v):
+                pages[self.tables[b, p // page], p % page] = rng.standard_normal((len(p), hk, d))
+        self.q = (scale * rng.standard_normal((n + pad, h, d))).astype(np.float32)
+        if bf16:
+            self.q = ref.round_bf16(self.q)
+            for pages in (self.k, self.v):
+                live = np.isfinite(pages)
+                pages[live] = ref.round_bf16(pages[live])
+        self.masks, self.positions = None, np.concatenate([c + np.arange(k) for c, k in zip(cached, new)] + [np.zeros(pad)]).astype(np.int64)
+        if tree:
+            words = -(-int(max(new)) // 32) + words_more
+            plan = ref.plan(cached, new, np.arange(pool + 9), 0, np.zeros((len(cached), int(total.max()) + 1), np.int64), page, n + pad, tree_parents(rng, new), words)
+            self.masks, self.positions = plan[3], plan[2]
+
+    def slot(self, b, p):
+        return int(self.tables[b, p // self.page]), p % self.page
+
+    def run(self, be, window=None, use_positions=True, workspace=False, heads_first=False, order=None, q_pad=0, kp=None, vp=None):
+        """(out, lse) as numpy; rows behind the last token keep 7."""
+        q, _ = strided(be, self.q, self.bf16, q_pad)
+        pages_order = (0, 2, 1, 3) if heads_first else None
+        kp = kp or strided(be, self.k, self.bf16, 0, pages_order)[0]
+        vp = vp or strided(be, self.v, self.bf16, 0, pages_order)[0]
+        out, base = strided(be, np.full(self.q.shape, 7.0, np.float32), self.bf16, q_pad)
+        lse = be.upload(np.full(self.q.shape[:2], 7.0, np.float32))
+        be.paged_attention_forward(q, kp, vp, u32(be, self.tables), u32(be, self.cached), u32(be, self.starts), masks=be.upload(self.masks) if self.masks is not None else None,
+                                   positions=u32(be, self.positions) if use_positions else None, window=window, out=out, lse=lse,
+                                   workspace=be.paged_attention_workspace(q, kp) if workspace else None)
+        be.sync()
+        return base.numpy()[..., : self.q.shape[2]], lse.numpy()
+
+    def check(self, be, window=None, use_positions=True, **kw):
+        got, lse = self.run(be, window, use_positions, **kw)
+        half = HALF_BF16 if self.bf16 else HALF_F32
+        n = int(self.starts[-1])
+        # unseen places are NaN: the reference looks at none of them either
+        want, want_lse, tol, lse_tol = ref.attention(self.q[:n], self.k, self.v, self.tables, self.cached, self.starts, self.masks, self.positions if use_positions else None, window,
+                                                     eps_out=half, eps_p=HALF_BF16 if self.bf16 else 0.0)
+        assert np.all(np.abs(got[:n] - want) <= tol), float((np.abs(got[:n] - want) / tol).max())
+        blank = np.isneginf(want_lse)
+        assert np.array_equal(np.isneginf(lse[:n]), blank) and not got[:n][blank].any()
+        assert np.all(np.abs(lse[:n][~blank] - want_lse[~blank]) <= lse_tol[~blank])
+        assert np.all(got[n:] == 7.0) and np.all(lse[n:] == 7.0)
+        return got, lse
+
+
+SHAPES = [  # cached, new, heads, KV heads, dim, page
+    ([0], [1], 1, 1, 64, 16), ([1], [1], 4, 4, 64, 16), ([776], [1], 12, 12, 64, 16), ([63, 64, 65], [1, 1, 1], 8, 2, 128, 16), ([127, 0, 300], [1, 5, 33], 4, 1, 128, 20),
+    ([500, 17], [9, 16], 8, 1, 64, 64), ([250], [63], 4, 4, 128, 32), ([200, 100], [128, 70], 8, 2, 64, 8), ([90], [130], 6, 2, 128, 16), ([33, 5], [3, 4], 6, 3, 96, 7),
+    ([40], [5], 2, 2, 80, 16), ([40, 2], [5, 31], 2, 1, 256, 16), ([31], [2], 3, 3, 66, 1), ([70], [6], 2, 2, 33, 5), ([1500, 1, 700], [17, 2, 0], 16, 2, 128, 64),
+    ([0, 0], [40, 64], 4, 2, 64, 16), ([260], [65], 16, 2, 128, 128), ([300], [128], 16, 1, 64, 24)]
+
+
+@pytest.mark.parametrize("cached,new,h,hk,d,page", SHAPES)
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("tree", [True, False])
+def test_attention(be, cached, new, h, hk, d, page, bf16, tree):
+    Case(len(cached) + d, cached, new, h, hk, d, page, tree, bf16, pad=2).check(be)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 100, 5000])
+@pytest.mark.parametrize("cached,new,h,hk,d,page", [SHAPES[i] for i in (1, 3, 4, 6, 9, 14)])
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("tree", [True, False])
+def test_attention_in_a_window(be, cached, new, h, hk, d, page, window, bf16, tree):
+    Case(window, cached, new, h, hk, d, page, tree, bf16).check(be, window=window)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("h,hk,d", [(8, 2, 128), (4, 4, 64), (3, 1, 40)])
+def test_attention_layouts_and_workspaces_give_the_same_bits(be, bf16, h, hk, d):
+    c = Case(5, [130, 7, 400], [9, 1, 20], h, hk, d, 16, True, bf16, words_more=1)
+    out, lse = c.check(be)
+    for kw in (dict(heads_first=True), dict(workspace=True), dict(q_pad=8, workspace=True)):
+        again = c.check(be, **kw)
+        assert np.array_equal(again[0], out) and np.array_equal(again[1], lse), kw
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("h,hk,d,new", [(4, 1, 64, [12, 3]), (2, 2, 128, [40, 1]), (8, 1, 128, [60, 33]), (3, 3, 48, [9, 9])])
+def test_attention_rows_that_see_nothing_and_poisoned_places_that_a_row_does_not_see(be, bf16, h, hk, d, new):
+    """Drafts that no row sees hold NaN and infinities; a row whose mask is empty over an empty cache is 0 with lse -inf; no fault is raised."""
+    c = Case(7, [0, 50], new, h, hk, d, 16, True, bf16)
+    c.masks[:] &= np.uint32(0xFFFFFFF5)                    # drafts 1 and 3 of each request drop out of every row
+    c.masks[0] = 0                                         # request 0 has no cache: its row 0 sees nothing
+    for b in range(2):
+        for j, bad in ((1, np.nan), (3, np.inf)):
+            if j < new[b]:
+                p, off = c.slot(b, int(c.cached[b]) + j)
+                c.k[p, off], c.v[p, off] = bad, -bad
+    out, lse = c.check(be)
+    assert not out[0].any() and np.all(np.isneginf(lse[0]))
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("h,hk,d,new,cached", [(4, 2, 64, 12, 20), (8, 1, 128, 40, 300), (2, 2, 48, 5, 10)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_poisoned_value_reaches_the_rows_that_see_it_and_no_other(be, bf16, h, hk, d, new, cached, bad):
+    from ojas_b200 import OjasError
+    c = Case(8, [cached], [new], h, hk, d, 16, True, bf16)
+    clean, clean_lse = c.check(be)
+    j = new // 2
+    p, off = c.slot(0, cached + j)
+    c.v[p, off, 0, 3] = bad
+    with pytest.raises(OjasError) as e:
+        c.run(be)
+    assert e.value.kind == "NonFinite" and "paged_attention" in str(e.value)
+    try:
+        got, lse = c.run(be)
+    except OjasError:
+        pass
+    q, _ = strided(be, c.q, bf16, 0)
+    out, lse_t = be.paged_attention_forward(q, floats(be, c.k, bf16), floats(be, c.v, bf16), u32(be, c.tables), u32(be, c.cached), u32(be, c.starts), masks=be.upload(c.masks),
+                                            positions=u32(be, c.positions))
+    with pytest.raises(OjasError):
+        be.sync()
+    got, lse = out.numpy(), lse_t.numpy()
+    sees = (c.masks[:, j // 32] >> np.uint32(j % 32) & 1).astype(bool)
+    heads = np.arange(h) < h // hk
+    assert np.array_equal(got[~sees], clean[~sees]) or np.abs(got[~sees] - clean[~sees]).max() <= (2.0 ** -7 if bf16 else 2.0 ** -18) * np.abs(clean).max()
+    assert np.all(np.isfinite(got[~sees])) and np.all(np.isfinite(got[:, ~heads]))
+    assert not np.any(np.isfinite(got[sees][:, heads, 3]))
+    # 1 x infinity is infinity, and a weight that underflows times infinity is NaN: either is what the formula gives
+    assert np.all(np.isfinite(got[sees][:, heads][..., 4:])) and np.array_equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("what", ["page", "length", "starts", "order"])
+def test_attention_reports_what_only_the_device_sees(be, bf16, what):
+    """Entries outside the pages, lengths beyond the table and starts beyond the rows: skipped, reported once, and the other requests' rows are right."""
+    from ojas_b200 import OjasError
+    c = Case(9, [100, 40], [4, 4], 4, 2, 64, 16, True, bf16)
+    clean, _ = c.check(be)
+    saved = c.tables.copy(), c.cached.copy(), c.starts.copy()
+    if what == "page":
+        c.tables[0, 2] = c.k.shape[0]
+    if what == "length":
+        c.cached[0] = 1 << 20
+    if what == "starts":
+        c.starts[2] = 4000
+    if what == "order":
+        c.starts[1] = 4000
+    q, _ = strided(be, c.q, bf16, 0)
+    out, _ = be.paged_attention_forward(q, floats(be, np.nan_to_num(c.k), bf16), floats(be, np.nan_to_num(c.v), bf16), u32(be, c.tables), u32(be, c.cached), u32(be, c.starts),
+                                        masks=be.upload(c.masks), positions=u32(be, c.positions))
+    with pytest.raises(OjasError) as e:
+        be.sync()
+    assert e.value.kind == "OutOfRange"
+    if what in ("page", "length"):
+        assert np.array_equal(out.numpy()[4:], clean[4:]) or np.abs(out.numpy()[4:] - clean[4:]).max() <= (2.0 ** -7 if bf16 else 2.0 ** -18) * np.abs(clean).max()
+    c.tables, c.cached, c.starts = saved
+    c.check(be)
+
+
+def test_attention_repeats_bit_for_bit(be):
+    c = Case(10, [3000, 900, 10], [40, 3, 64], 8, 2, 128, 16, True, True)
+    first = c.run(be)
+    for _ in range(3):
+        again = c.run(be)
+        assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+
+
+def test_cached_attention_agrees_with_the_paged_form(be):
+    """One sequence, causal drafts: the ring cache's op on the same keys (its span is the cache's whole length)."""
+    c = Case(11, [45], [3], 4, 2, 64, 16, tree=False, bf16=False)
+    out, _ = c.check(be)
+    p = np.arange(48)
+    kc, vc = (a[c.tables[0, p // 16], p % 16][None] for a in (c.k, c.v))
+    want = be.cached_attention_forward(be.upload(c.q[None]), be.upload(kc), be.upload(vc), 48).numpy()[0]
+    assert np.abs(out - want).max() <= 2.0 ** -16 * np.abs(want).max()
+
+
+# ---------------------------------------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_decoding_loop_over_pages(be, bf16):
+    """Prompts of different lengths, then trees of drafts of which one path is kept, then single tokens: at every pass the plan, q's rotation, the write
+    with k's rotation and the attention, against attention over the kept history rebuilt in 64 bits."""
+    from ojas_b200 import DType, RopeSpec
+    rng = np.random.default_rng(12)
+    h, hk, d, page, pool, width = 4, 2, 64, 8, 64, 16
+    plan, f = be.rope_plan(RopeSpec(d, layout="interleaved", scaling="linear", factor=2.0)), ref.frequencies(d, scaling="linear", factor=2.0)
+    dt = DType.BF16 if bf16 else DType.F32
+    kp, vp = floats(be, np.full((pool, page, hk, d), np.nan), bf16), floats(be, np.full((pool, page, hk, d), np.nan), bf16)
+    tables, free = u32(be, np.full((3, width), NONE)), u32(be, rng.permutation(pool))
+    head = u32(be, [0])
+    cached = np.zeros(3, np.int64)
+    keys = [np.zeros((0, hk, d)) for _ in range(3)]     # the history as the cache holds it: rotated, rounded
+    values = [np.zeros((0, hk, d)) for _ in range(3)]
+    half = HALF_BF16 if bf16 else HALF_F32
+    for new, tree in (([9, 1, 30], False), ([7, 7, 1], True), ([1, 1, 1], False), ([0, 5, 12], True), ([1, 1, 1], False)):
+        n, capacity = sum(new), sum(new) + 3
+        parents = np.concatenate([tree_parents(rng, new), np.zeros(3, np.int64)]) if tree else None
+        q, k, v = (rng.standard_normal((capacity, x, d)).astype(np.float32) for x in (h, hk, hk))
+        if bf16:
+            q, k, v = ref.round_bf16(q), ref.round_bf16(k), ref.round_bf16(v)
+        p = be.paged_plan(u32(be, cached), u32(be, new), free, head, tables, page, tokens=capacity, parents=u32(be, parents) if tree else None, mask_words=1 if tree else 0)
+        dq = be.rope_forward(floats(be, q, bf16), p.positions, plan)
+        be.paged_kv_write(kp, vp, floats(be, k, bf16), floats(be, v, bf16), p.slots, rope=plan, positions=p.positions)
+        out, _ = be.paged_attention_forward(dq, kp, vp, tables, u32(be, cached), p.starts, masks=p.masks, positions=p.positions, out=be.zeros((capacity, h, d), dt))
+        positions, starts = p.positions.numpy().astype(np.int64), p.starts.numpy()
+        got, rq = out.numpy(), dq.numpy()
+        rk = ref.rotate(k, positions, f, "interleaved")
+        rk = ref.round_bf16(rk) if bf16 else rk.astype(np.float32)
+        assert np.abs(rq[:n] - ref.rotate(q, positions, f, "interleaved")[:n]).max() <= rope_bound(q, None, 1.0, half)
+        longest = max(len(x) for x in keys) + max(new)
+        ck, cv = np.zeros((3, longest, hk, d), np.float32), np.zeros((3, longest, hk, d), np.float32)
+        for b in range(3):
+            s = slice(starts[b], starts[b + 1])
+            ck[b, :cached[b] + new[b]] = np.concatenate([keys[b], rk[s]])
+            cv[b, :cached[b] + new[b]] = np.concatenate([values[b], v[s]])
+        # the keys' own rounding differs by at most one step from the device's; q is compared as the device rotated it
+        want, _, tol, _ = ref.attention(rq[:n], ck, cv, np.arange(3)[:, None], cached, starts, p.masks.numpy() if tree else None, positions, None, half, HALF_BF16 if bf16 else 0.0)
+        slack = (2 * half + 2.0 ** -19) * np.abs(rk).max() * np.abs(rq[:n]).sum(-1, keepdims=True) / np.sqrt(d)
+        assert np.all(np.abs(got[:n] - want) <= tol + 2 * slack * np.abs(cv).max()) and not got[n:].any()
+        for b in range(3):                               # keep a path: the last draft's ancestors move to the front of the new places
+            kept = list(range(new[b]))
+            if tree and new[b]:
+                row = p.masks.numpy()[starts[b + 1] - 1, 0]
+                kept = [j for j in range(new[b]) if row >> j & 1]
+            slots = p.slots.numpy()[starts[b]:starts[b + 1]]
+            if kept != list(range(new[b])):
+                t = [starts[b] + j for j in kept]
+                be.paged_kv_write(kp, vp, floats(be, k[t], bf16), floats(be, v[t], bf16), u32(be, slots[: len(kept)]), rope=plan, positions=u32(be, positions[t]))
+            t = [starts[b] + j for j in kept]
+            keys[b], values[b] = np.concatenate([keys[b], rk[t]]), np.concatenate([values[b], v[t]])
+            cached[b] += len(kept)
+        head = u32(be, [int(p.free_head.numpy()[0])])    # pages of dropped drafts stay in their request's table
+    be.sync()
