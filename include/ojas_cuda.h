@@ -201,7 +201,8 @@ ojc_status ojc_cached_attention_forward(ojc_backend* be, const ojc_tensor* q, co
  *      paged_plan (once), rope_forward on q, paged_kv_write of k and v, paged_attention_forward; nothing in it is read back to the host, and shapes
  *      depend on capacities alone, so a pass may be captured from ojc_stream into a graph (replay it on that stream; give paged_attention_forward a
  *      workspace of the caller's). All index tensors are U32; OJC_NONE stands for "no slot" and "no parent". What the host cannot see is checked on
- *      the device: a page, slot, length or parent out of range is skipped and surfaces as OutOfRange at the next sync. */
+ *      the device: a page, slot, length, position or parent out of range is never followed and surfaces as OutOfRange at the next sync (the outputs of
+ *      its request are then unspecified, the other requests' are right). */
 #define OJC_NONE 0xffffffffu
 /* Block tables and slot maps from lengths. cached_lens, new_lens [B]; parents [N] (optional): draft i's parent as its index among the request's
  * own drafts, below i, or OJC_NONE for a child of the last cached token; without parents each token follows the one before it. New pages are taken from
@@ -235,7 +236,7 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
  * Head h reads KV head h / (H / Hkv), the scale is 1 / sqrt(D). Token i of request b sees the cached places below cached_lens[b] and, of the
  * request's new tokens, those whose bits are set in row i of masks [N, words], or without masks those up to itself; of all these, with window >= 1,
  * only those whose position is above its own minus window (the position of a cached place is the place, that of a new token its entry of positions
- * [N]; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). Masked places are never
+ * [N], at least the cached length; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). Masked places are never
  * looked at: NaN or infinity there does no harm. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
  * non-finite value that a row does see surfaces as NonFinite. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
  * NULL for the library's own (refused while the stream is being captured). */

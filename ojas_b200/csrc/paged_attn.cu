@@ -2,6 +2,8 @@
 //
 // out_i = sum_j p_ij v_j, p_ij = exp(s_ij - max_j s_ij) / sum, s_ij = q_i . k_j / sqrt(D) over the places j that row i sees: the cached ones inside
 // its window, and of its request's new tokens those in its ancestor mask (or up to itself). One pass over the keys with a running maximum and sum.
+#include <type_traits>
+
 #include "dispatch.cuh"
 #include "paged.cuh"
 
@@ -44,6 +46,7 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
   const int64_t fresh = bad ? 0 : end - first, total = bad ? 0 : cached + fresh;
   const int64_t place = ix.positions ? ix.positions[t] : cached + local;
   const int64_t low = ix.window > 0 ? place - ix.window : -1;   // keys at positions above `low` are in the window
+  bad |= ix.window > 0 && place < cached;
   float* qs = sm + warp * dim;
   const T* qp = q.ptr + t * q.sn + h * q.sh;
   for (int d = lane; d < dim; d += 32) qs[d] = ldf(qp, d);
@@ -111,6 +114,544 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
   else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
 }
 
+// ======================================================================== tiles on the tensor cores
+// A unit of work is (request, KV head, row tile): the rows of a KV head are its request's tokens times the query heads of the group (token-major), cut
+// into tiles of 16 * MW; its keys are walked in blocks of 64. All units' blocks in a row are one line of work that the CTAs share out evenly, whatever
+// the lengths: a CTA that gets the middle of a unit leaves (maximum, sum, unnormalised output) per row in the workspace, and a second small kernel joins
+// the pieces of a unit in order. Every CTA finds its own stretch from the lengths, so nothing is planned on the host and nothing read back.
+//
+// What bounds it: the cache's bytes for few rows. Four warps to a CTA, two CTAs to an SM, three stages of 64 keys each, rows fetched by 16-byte asynchronous
+// copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
+// out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
+// Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
+constexpr int BLOCK_KEYS = 64, TILE_WARPS = 4;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {   // zeros when the source is not there
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+// x = hi + lo up to 2^-22 |x|, both TF32
+__device__ __forceinline__ void split_tf32(float x, uint32_t* hi, uint32_t* lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*lo) : "f"(x - __uint_as_float(*hi)));
+}
+__device__ __forceinline__ float quad_max(float v) { v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1)); return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)); }
+__device__ __forceinline__ float quad_sum(float v) { v += __shfl_xor_sync(0xffffffffu, v, 1); return v + __shfl_xor_sync(0xffffffffu, v, 2); }
+
+// What a unit that several CTAs share leaves for the joining kernel: its pieces are slot 2c + 1 of its first CTA c and slots 2(c + 1), 2(c + 2), ...
+struct SplitUnit { int pieces, request, kv_head, row_tile; };
+struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][16 MW][D], ml [2 CTAs][16 MW], split [CTAs]
+
+struct Request { int64_t cached; uint32_t first; int fresh, first_block, blocks, row_tiles; };
+__device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int group, int tile_rows, bool* bad) {
+  Request r;
+  const uint32_t first = ix.starts[b], end = ix.starts[b + 1];
+  r.cached = ix.cached[b];
+  r.first = first;
+  const bool wrong = end < first || end > ix.tokens || r.cached + (int64_t)(end - first) > ix.width * ix.page;
+  *bad |= wrong;
+  r.fresh = wrong ? 0 : (int)(end - first);
+  const int64_t from = ix.window > 0 ? max((int64_t)0, r.cached - ix.window + 1) : 0;   // positions of new tokens are at least `cached`
+  r.first_block = (int)(from / BLOCK_KEYS);
+  r.blocks = (int)((r.cached + r.fresh + BLOCK_KEYS - 1) / BLOCK_KEYS) - r.first_block;
+  r.row_tiles = (r.fresh * group + tile_rows - 1) / tile_rows;
+  if (r.fresh == 0) r.blocks = 0;
+  return r;
+}
+
+// A place on the line of work; all threads of a CTA hold the same one.
+struct Cursor {
+  Request r;
+  int b, unit, block;     // unit: kv_head * row_tiles + row_tile; block counts from 0
+  __device__ __forceinline__ void step(const PassIndex& ix, int group, int tile_rows, int kv_heads, bool* bad) {
+    if (++block < r.blocks) return;
+    block = 0;
+    if (++unit < kv_heads * r.row_tiles) return;
+    unit = 0;
+    do { if (++b >= ix.batch) return; r = load_request(ix, b, group, tile_rows, bad); } while (r.blocks == 0);
+  }
+};
+
+template <class T, int D, int MW> struct TileShape {
+  static constexpr int K_PITCH = std::is_same<T, float>::value ? D + 4 : D + 8, V_PITCH = D + 8;   // elements: odd multiples of 16 bytes (ldmatrix), or 4 and 8 banks a row (F32 fragments)
+  static constexpr int STAGE = BLOCK_KEYS * (K_PITCH + V_PITCH) * (int)sizeof(T);
+  static constexpr bool Q_IN_REGS = std::is_same<T, bf16>::value && D <= 128;
+  static constexpr int JOINT = MW < TILE_WARPS ? 16 * (D + 2) * 4 : 0, OFFSETS = TILE_WARPS * 32 * 8, Q_TILE = Q_IN_REGS ? 0 : 16 * MW * K_PITCH * (int)sizeof(T);
+  static constexpr int STAGES = 3 * STAGE + JOINT + OFFSETS + Q_TILE <= 226 * 1024 ? 3 : 2;          // what an SM holds
+  static constexpr int SMEM = STAGES * STAGE + JOINT + OFFSETS + Q_TILE;
+  static constexpr int CTAS_PER_SM = SMEM <= 112 * 1024 + 512 ? 2 : 1;
+};
+
+template <class T, int D, int MW>
+__global__ void __launch_bounds__(TILE_WARPS * 32, TileShape<T, D, MW>::CTAS_PER_SM)
+paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesView<const T> vp, PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads,
+                             int group, int kv_heads, float scale, uint32_t* fault) {
+  using S = TileShape<T, D, MW>;
+  constexpr bool F32 = std::is_same<T, float>::value;
+  constexpr int STAGES = S::STAGES;
+  constexpr int KW = TILE_WARPS / MW, KEYS = BLOCK_KEYS / KW, NT = KEYS / 8, OT = D / 8, TILE_ROWS = 16 * MW;
+  constexpr int CHUNKS = D * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
+  constexpr int KSTEP = F32 ? 8 : 16, KSTEPS = D / KSTEP;
+  extern __shared__ __align__(128) uint8_t raw[];
+  float* joint = reinterpret_cast<float*>(raw + STAGES * S::STAGE);                                   // [16][D] and [16] (m, l): the warps' outputs meet here
+  int64_t* offsets = reinterpret_cast<int64_t*>(raw + STAGES * S::STAGE + S::JOINT);
+  T* q_tile = reinterpret_cast<T*>(offsets + TILE_WARPS * 32);                                          // only without Q_IN_REGS
+  __shared__ unsigned long long s_sum[TILE_WARPS], s_at;
+  __shared__ int s_b;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
+  bool bad = false, wrong = false;
+
+  // ---- this CTA's stretch [begin, end) of the line of work
+  unsigned long long total = 0;
+  for (int b = tid; b < ix.batch; b += TILE_WARPS * 32) {
+    const Request r = load_request(ix, b, group, TILE_ROWS, &bad);
+    total += (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
+  }
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s_sum[warp] = total;
+  __syncthreads();
+  total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  const unsigned long long ctas = min((unsigned long long)gridDim.x, (total + 1) / 2);                  // at least two blocks each
+  if (tid == 0) work.split[blockIdx.x] = SplitUnit{0, 0, 0, 0};
+  if (bad) raise_fault(fault, OP_PAGED_RANGE);
+  if (blockIdx.x >= ctas) return;
+  const unsigned long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
+  unsigned long long carry = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {                                              // the request that holds `begin`
+    const int b = b0 + tid;
+    unsigned long long n = 0;
+    if (b < ix.batch) { const Request r = load_request(ix, b, group, TILE_ROWS, &bad); n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads); }
+    unsigned long long sum = n;
+    for (int o = 1; o < 32; o <<= 1) { const unsigned long long a = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += a; }
+    if (lane == 31) s_sum[warp] = sum;
+    __syncthreads();
+    unsigned long long at = carry + sum - n;
+    for (int w = 0; w < TILE_WARPS; ++w) { if (w < warp) at += s_sum[w]; carry += s_sum[w]; }
+    if (n && at <= begin && begin < at + n) { s_b = b; s_at = at; }
+    __syncthreads();
+    if (carry > begin) break;
+  }
+  Cursor use;
+  use.b = s_b;
+  use.r = load_request(ix, use.b, group, TILE_ROWS, &bad);
+  use.unit = (int)((begin - s_at) / (unsigned)use.r.blocks);
+  use.block = (int)((begin - s_at) % (unsigned)use.r.blocks);
+  Cursor ahead = use;                                                                                   // the block whose pages are looked up next
+  const int64_t todo = (int64_t)(end - begin);
+
+  // ---- copies: warp w fetches keys 16 w .. 16 w + 15 of a block; lane l < 16 looks up key l's place
+  uint32_t id = 0, off = 0;
+  int hk_ahead = 0;
+  bool there = false;
+  auto look_up = [&]() {
+    const int64_t j = (int64_t)(ahead.r.first_block + ahead.block) * BLOCK_KEYS + 16 * warp + (lane & 15);
+    there = j < ahead.r.cached + ahead.r.fresh;
+    hk_ahead = ahead.unit / ahead.r.row_tiles;
+    if (there) {
+      const uint32_t pi = (uint32_t)j / ix.page;
+      off = (uint32_t)j - pi * ix.page;
+      id = ix.tables[(int64_t)ahead.b * ix.width + pi];
+    }
+    ahead.step(ix, group, TILE_ROWS, kv_heads, &bad);
+  };
+  int64_t* my_offsets = offsets + warp * 32;
+  auto copy_block = [&](int stage) {
+    if (there && id >= ix.pages) { bad = true; there = false; }
+    my_offsets[lane] = !there ? -1 : lane < 16 ? id * kp.sp + off * kp.st + hk_ahead * kp.sh : id * vp.sp + off * vp.st + hk_ahead * vp.sh;
+    __syncwarp();
+    const uint32_t base = smem_addr(raw) + stage * S::STAGE + (16 * warp) * S::K_PITCH * (int)sizeof(T);
+    const uint32_t vbase = smem_addr(raw) + stage * S::STAGE + (BLOCK_KEYS * S::K_PITCH + 16 * warp * S::V_PITCH) * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < CHUNKS / 2; ++i) {
+      const int at = lane + 32 * i, row = at / CHUNKS, c = at % CHUNKS;
+      const int64_t ko = my_offsets[row];
+      copy16(base + row * S::K_PITCH * (int)sizeof(T) + c * 16, kp.ptr + (ko < 0 ? 0 : ko) + c * PER, ko >= 0);
+    }
+#pragma unroll
+    for (int i = 0; i < CHUNKS / 2; ++i) {
+      const int at = lane + 32 * i, row = at / CHUNKS, c = at % CHUNKS;
+      const int64_t vo = my_offsets[16 + row];
+      copy16(vbase + row * S::V_PITCH * (int)sizeof(T) + c * 16, vp.ptr + (vo < 0 ? 0 : vo) + c * PER, vo >= 0);
+    }
+    __syncwarp();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (s < todo) { copy_block(s); if (s + 1 < todo) look_up(); }
+    copies_commit();
+  }
+
+  uint32_t qf[S::Q_IN_REGS ? KSTEPS : 1][4];
+  float o[OT][4], m[2], l[2];
+  bool any[2];
+  int64_t low[2], low_most = -1;
+  int local[2];
+  bool live[2];
+  const float c2 = scale * 1.4426950408889634f;
+  unsigned long long piece_begin = begin;
+
+  for (int64_t f = 0; f < todo; ++f) {
+    const int row_tile = use.unit % use.r.row_tiles, hk = use.unit / use.r.row_tiles;
+    if (f == 0 || use.block == 0) {                                                                     // a new unit: its rows
+      piece_begin = begin + f;
+      low_most = -1;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = row_tile * TILE_ROWS + 16 * mw + quad + 8 * x;
+        live[x] = r < use.r.fresh * group;
+        local[x] = live[x] ? r / group : 0;
+        const int64_t t = use.r.first + local[x];
+        const int64_t place = ix.positions ? (int64_t)ix.positions[t] : use.r.cached + local[x];
+        low[x] = ix.window > 0 ? place - ix.window : -1;
+        if (live[x] && ix.window > 0 && place < use.r.cached) bad = true;
+        if (live[x]) low_most = max(low_most, low[x]);
+        m[x] = -INFINITY; l[x] = 0.0f; any[x] = false;
+        if (S::Q_IN_REGS) {
+          const uint32_t* p = reinterpret_cast<const uint32_t*>(q.ptr + t * q.sn + (int64_t)(hk * group + (live[x] ? r % group : 0)) * q.sh);
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) { qf[k][x] = live[x] ? p[8 * k + pair] : 0u; qf[k][2 + x] = live[x] ? p[8 * k + 4 + pair] : 0u; }
+        }
+      }
+      if (ix.window > 0) for (int s = 16; s > 0; s >>= 1) low_most = max(low_most, __shfl_xor_sync(0xffffffffu, low_most, s));
+      if (!S::Q_IN_REGS) {
+        __syncthreads();
+        for (int i = tid; i < TILE_ROWS * CHUNKS; i += TILE_WARPS * 32) {
+          const int r = i / CHUNKS, c = i % CHUNKS, g = row_tile * TILE_ROWS + r;
+          const bool has = g < use.r.fresh * group;
+          const T* p = q.ptr + (int64_t)(use.r.first + (has ? g / group : 0)) * q.sn + (int64_t)(hk * group + (has ? g % group : 0)) * q.sh + c * PER;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (has) v = *reinterpret_cast<const uint4*>(p);
+          *reinterpret_cast<uint4*>(q_tile + r * S::K_PITCH + c * PER) = v;
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int n = 0; n < OT; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
+    }
+
+    copies_wait<STAGES - 2>();
+    if (MW == 1) __syncwarp(); else __syncthreads();
+    {                                                                                                   // the stage that the last block left
+      const int64_t next = f + STAGES - 1;
+      if (next < todo) { copy_block((int)(next % STAGES)); if (next + 1 < todo) look_up(); }
+      copies_commit();
+    }
+    const int stage = (int)(f % STAGES);
+    const T* kt = reinterpret_cast<const T*>(raw + stage * S::STAGE) + kw * KEYS * S::K_PITCH;
+    const T* vt = reinterpret_cast<const T*>(raw + stage * S::STAGE) + BLOCK_KEYS * S::K_PITCH + kw * KEYS * S::V_PITCH;
+    const int64_t j0 = (int64_t)(use.r.first_block + use.block) * BLOCK_KEYS + kw * KEYS;
+
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f; }
+    if (!F32) {
+      const uint32_t ka = smem_addr(kt) + ((((lane >> 4) & 1) * 8 + (lane & 7)) * S::K_PITCH + ((lane >> 3) & 1) * 8) * 2;
+      const uint32_t qa = smem_addr(q_tile) + ((16 * mw + (lane & 15)) * S::K_PITCH + (lane >> 4) * 8) * 2;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        uint32_t a[4];
+        if (S::Q_IN_REGS) { a[0] = qf[k][0]; a[1] = qf[k][1]; a[2] = qf[k][2]; a[3] = qf[k][3]; }
+        else ldmatrix4(a, qa + k * 32);
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b4[4];
+          ldmatrix4(b4, ka + (n * 8 * S::K_PITCH + k * 16) * 2);
+          mma_bf16(s[n], a, b4[0], b4[1]);
+          mma_bf16(s[n + 1], a, b4[2], b4[3]);
+        }
+      }
+    } else {
+      const float* qa = reinterpret_cast<const float*>(q_tile) + (16 * mw + quad) * S::K_PITCH + pair;
+      const float* ka = reinterpret_cast<const float*>(kt) + quad * S::K_PITCH + pair;
+#pragma unroll 4
+      for (int k = 0; k < KSTEPS; ++k) {
+        uint32_t ah[4], al[4];
+        split_tf32(qa[8 * k], &ah[0], &al[0]); split_tf32(qa[8 * S::K_PITCH + 8 * k], &ah[1], &al[1]);
+        split_tf32(qa[8 * k + 4], &ah[2], &al[2]); split_tf32(qa[8 * S::K_PITCH + 8 * k + 4], &ah[3], &al[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t bh0, bl0, bh1, bl1;
+          split_tf32(ka[n * 8 * S::K_PITCH + 8 * k], &bh0, &bl0); split_tf32(ka[n * 8 * S::K_PITCH + 8 * k + 4], &bh1, &bl1);
+          mma_tf32(s[n], al, bh0, bh1);
+          mma_tf32(s[n], ah, bl0, bl1);
+          mma_tf32(s[n], ah, bh0, bh1);
+        }
+      }
+    }
+
+    // ---- what the rows see: everything in a block below the cached length and inside every row's window
+    uint32_t sees = 0xffffffffu;                                                                        // bit 4 n + element
+    bool poisoned = false;
+    if (j0 + KEYS > use.r.cached || (ix.window > 0 && j0 <= low_most)) {
+      sees = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = e >> 1;
+          const int64_t j = j0 + 8 * n + 2 * pair + (e & 1);
+          bool v = live[x];
+          if (j < use.r.cached) v = v && j > low[x];
+          else {
+            const uint32_t d = (uint32_t)(j - use.r.cached);
+            v = v && d < (uint32_t)use.r.fresh;
+            if (v) v = ix.masks ? (d >> 5) < (uint32_t)ix.words && (ix.masks[(int64_t)(use.r.first + local[x]) * ix.words + (d >> 5)] >> (d & 31) & 1u) : d <= (uint32_t)local[x];
+            if (v && ix.window > 0) v = (ix.positions ? (int64_t)ix.positions[use.r.first + d] : j) > low[x];
+          }
+          if (v) sees |= 1u << (4 * n + e); else s[n][e] = -INFINITY;
+        }
+      }
+      // a value that only some rows see must not reach the others as 0 x NaN: such a block's second product goes without the tensor cores
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(vt);
+      constexpr int WORDS = D * (int)sizeof(T) / 4, PITCH_WORDS = S::V_PITCH * (int)sizeof(T) / 4;
+      for (int i = lane; i < KEYS * WORDS; i += 32) {
+        const uint32_t x = w[(i / WORDS) * PITCH_WORDS + i % WORDS];
+        if (F32) poisoned |= (x & 0x7f800000u) == 0x7f800000u;
+        else poisoned |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+      }
+      poisoned = __any_sync(0xffffffffu, poisoned);
+    }
+
+    // ---- running maximum and sum
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][2 * x], s[n][2 * x + 1]));
+      top = fmaxf(m[x], quad_max(top));
+      const float base = top == -INFINITY ? 0.0f : top * c2;
+      const float corr = exp2_fast(fmaf(m[x], c2, -base));
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][2 * x] = exp2_fast(fmaf(s[n][2 * x], c2, -base));
+        s[n][2 * x + 1] = exp2_fast(fmaf(s[n][2 * x + 1], c2, -base));
+        sum += s[n][2 * x] + s[n][2 * x + 1];
+      }
+      any[x] |= (sees & (0x33333333u << (2 * x)) & (NT == 8 ? 0xffffffffu : (1u << (4 * NT & 31)) - 1u)) != 0;
+      if (__any_sync(0xffffffffu, top != m[x])) {
+#pragma unroll
+        for (int n = 0; n < OT; ++n) { o[n][2 * x] *= corr; o[n][2 * x + 1] *= corr; }
+      }
+      l[x] = l[x] * corr + sum;
+      m[x] = top;
+    }
+
+    // ---- O += P V
+    if (poisoned) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) {
+          const int from = (lane & ~3) | (k >> 1);
+          float p[2];
+          bool v[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            p[x] = __shfl_sync(0xffffffffu, (k & 1) ? s[n][2 * x + 1] : s[n][2 * x], from);
+            v[x] = __shfl_sync(0xffffffffu, sees >> (4 * n + 2 * x + (k & 1)) & 1u, from);
+          }
+#pragma unroll
+          for (int i = 0; i < OT; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float val = ldf(vt, (8 * n + k) * S::V_PITCH + 8 * i + 2 * pair + (e & 1));
+              if (v[e >> 1]) o[i][e] = fmaf(p[e >> 1], val, o[i][e]);
+            }
+          }
+        }
+      }
+    } else if (!F32) {
+      const uint32_t va = smem_addr(vt) + ((((lane >> 3) & 1) * 8 + (lane & 7)) * S::V_PITCH + ((lane >> 4) & 1) * 8) * 2;
+#pragma unroll
+      for (int k = 0; k < NT / 2; ++k) {
+        const uint32_t a[4] = {pack_bf16(s[2 * k][0], s[2 * k][1]), pack_bf16(s[2 * k][2], s[2 * k][3]), pack_bf16(s[2 * k + 1][0], s[2 * k + 1][1]),
+                               pack_bf16(s[2 * k + 1][2], s[2 * k + 1][3])};
+#pragma unroll
+        for (int n = 0; n < OT; n += 2) {
+          uint32_t b4[4];
+          ldmatrix4_trans(b4, va + (k * 16 * S::V_PITCH + n * 8) * 2);
+          mma_bf16(o[n], a, b4[0], b4[1]);
+          mma_bf16(o[n + 1], a, b4[2], b4[3]);
+        }
+      }
+    } else {
+      // the k index of the product runs over keys in the order 0 2 4 6 1 3 5 7 of a tile of eight: the order in which the scores lie in the registers
+      const float* va = reinterpret_cast<const float*>(vt) + 2 * pair * S::V_PITCH + quad;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        uint32_t ah[4], al[4];
+        split_tf32(s[k][0], &ah[0], &al[0]); split_tf32(s[k][2], &ah[1], &al[1]); split_tf32(s[k][1], &ah[2], &al[2]); split_tf32(s[k][3], &ah[3], &al[3]);
+#pragma unroll
+        for (int n = 0; n < OT; ++n) {
+          uint32_t bh0, bl0, bh1, bl1;
+          split_tf32(va[k * 8 * S::V_PITCH + 8 * n], &bh0, &bl0); split_tf32(va[(k * 8 + 1) * S::V_PITCH + 8 * n], &bh1, &bl1);
+          mma_tf32(o[n], al, bh0, bh1);
+          mma_tf32(o[n], ah, bl0, bl1);
+          mma_tf32(o[n], ah, bh0, bh1);
+        }
+      }
+    }
+
+    // ---- the end of the unit, or of this CTA's piece of it
+    const bool unit_done = use.block + 1 == use.r.blocks;
+    if (unit_done || f + 1 == todo) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        l[x] = quad_sum(l[x]);
+        int seen = any[x];
+        seen |= __shfl_xor_sync(0xffffffffu, seen, 1); seen |= __shfl_xor_sync(0xffffffffu, seen, 2);
+        if (seen && m[x] == -INFINITY) l[x] = NAN;                                                      // every score -inf: what the formula gives
+      }
+      if (KW > 1) {                                                                                     // the warps that share a row tile add up in order
+        float* jm = joint + 16 * D;
+        for (int w = 1; w < KW; ++w) {
+          for (int g = 0; g < MW; ++g) {
+            __syncthreads();
+            if (kw == w && mw == g) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int r = quad + 8 * x;
+                if (pair == 0) { jm[2 * r] = m[x]; jm[2 * r + 1] = l[x]; }
+#pragma unroll
+                for (int n = 0; n < OT; ++n) *reinterpret_cast<float2*>(joint + r * D + 8 * n + 2 * pair) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+              }
+            }
+            __syncthreads();
+            if (kw == 0 && mw == g) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int r = quad + 8 * x;
+                const float m2 = jm[2 * r], l2 = jm[2 * r + 1], top = fmaxf(m[x], m2), base = top == -INFINITY ? 0.0f : top * c2;
+                const float ca = exp2_fast(fmaf(m[x], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
+                l[x] = l[x] * ca + l2 * cb;
+                m[x] = top;
+#pragma unroll
+                for (int n = 0; n < OT; ++n) {
+                  const float2 v = *reinterpret_cast<const float2*>(joint + r * D + 8 * n + 2 * pair);
+                  o[n][2 * x] = o[n][2 * x] * ca + v.x * cb;
+                  o[n][2 * x + 1] = o[n][2 * x + 1] * ca + v.y * cb;
+                }
+              }
+            }
+          }
+        }
+      }
+      const unsigned long long unit_begin = begin + f - use.block;                                      // wraps below zero never: a unit's blocks are on the line
+      const bool whole = unit_done && piece_begin == unit_begin;
+      if (kw == 0) {
+        const int slot = 2 * blockIdx.x + (piece_begin == unit_begin ? 1 : 0);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (!live[x]) continue;
+          const int r = row_tile * TILE_ROWS + 16 * mw + quad + 8 * x;
+          const int64_t t = use.r.first + local[x];
+          const int h = hk * group + r % group;
+          if (whole) {
+            const bool seen = !(m[x] == -INFINITY && l[x] == 0.0f);
+            const float inv = seen ? 1.0f / l[x] : 0.0f;
+            T* p = out.ptr + t * out.sn + h * out.sh;
+#pragma unroll
+            for (int n = 0; n < OT; ++n) {
+              const float u = o[n][2 * x] * inv, v = o[n][2 * x + 1] * inv;
+              wrong |= !isfinite(u) || !isfinite(v);
+              if (F32) *reinterpret_cast<float2*>(p + 8 * n + 2 * pair) = make_float2(u, v);
+              else *reinterpret_cast<uint32_t*>(p + 8 * n + 2 * pair) = pack_bf16(u, v);
+            }
+            if (pair == 0 && lse) lse[t * heads + h] = seen ? m[x] * scale + logf(l[x]) : -INFINITY;
+          } else {
+            const int64_t row = (int64_t)slot * TILE_ROWS + 16 * mw + quad + 8 * x;
+            if (pair == 0) work.ml[row] = make_float2(m[x], l[x]);
+#pragma unroll
+            for (int n = 0; n < OT; ++n) *reinterpret_cast<float2*>(work.o + row * D + 8 * n + 2 * pair) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+          }
+        }
+      }
+      if (!unit_done && piece_begin == unit_begin && tid == 0) {                                        // this CTA holds the unit's first piece
+        const unsigned long long unit_end = unit_begin + use.r.blocks, last = (unit_end * ctas + total - 1) / total - 1;
+        work.split[blockIdx.x] = SplitUnit{(int)(last - blockIdx.x) + 1, use.b, hk, row_tile};
+      }
+    }
+    use.step(ix, group, TILE_ROWS, kv_heads, &bad);
+  }
+  if (bad) raise_fault(fault, OP_PAGED_RANGE);
+  else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
+}
+
+// Joins the pieces of the units that several CTAs shared: block (c, row) takes row `row` of the unit whose first piece CTA c left. Four warps walk the
+// pieces (a fixed order), lanes the columns.
+template <class T>
+__global__ void __launch_bounds__(128)
+paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, float scale, uint32_t* fault) {
+  __shared__ float acc[4][256], s_l[4], s_m[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const SplitUnit u = work.split[blockIdx.x];
+  if (u.pieces == 0) return;
+  const uint32_t first = ix.starts[u.request];
+  const int r = u.row_tile * tile_rows + blockIdx.y;
+  if (r >= (int)(ix.starts[u.request + 1] - first) * group) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float c2 = scale * 1.4426950408889634f;
+  auto row_of = [&](int p) { return (int64_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * tile_rows + blockIdx.y; };
+  float top = -INFINITY;
+  for (int p = tid; p < u.pieces; p += 128) top = fmaxf(top, work.ml[row_of(p)].x);
+  top = warp_max(top);
+  if (lane == 0) s_m[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float base = top == -INFINITY ? 0.0f : top * c2;
+  float l = 0.0f, o[MAXI];
+#pragma unroll
+  for (int i = 0; i < MAXI; ++i) o[i] = 0.0f;
+#pragma unroll 4
+  for (int p = warp; p < u.pieces; p += 4) {
+    const int64_t row = row_of(p);
+    const float2 ml = work.ml[row];
+    const float w = exp2_fast(fmaf(ml.x, c2, -base));
+    l = fmaf(ml.y, w, l);
+#pragma unroll
+    for (int i = 0; i < MAXI; ++i) { const int d = lane + 32 * i; if (d < dim) o[i] = fmaf(work.o[row * dim + d], w, o[i]); }
+  }
+#pragma unroll
+  for (int i = 0; i < MAXI; ++i) { const int d = lane + 32 * i; if (d < dim) acc[warp][d] = o[i]; }
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  const bool seen = !(top == -INFINITY && l == 0.0f);
+  const float inv = seen ? 1.0f / l : 0.0f;
+  const int64_t t = first + r / group;
+  const int h = u.kv_head * group + r % group;
+  T* po = out.ptr + t * out.sn + h * out.sh;
+  bool wrong = false;
+  for (int d = tid; d < dim; d += 128) {
+    const float v = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
+    wrong |= !isfinite(v);
+    stf(po, d, v);
+  }
+  if (tid == 0 && lse) lse[t * heads + h] = seen ? top * scale + logf(l) : -INFINITY;
+  if (wrong) raise_fault(fault, OP_PAGED_ATTN);
+}
+
 ojc_status u32_table(const char* op, const char* what, const ojc_tensor* t, int rank) {
   OJC_TRY(check_tensor(op, what, t));
   if (t->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, std::string(what) + " is U32");
@@ -132,6 +673,75 @@ ojc_status attn_dims(const char* op, const ojc_tensor* q, const ojc_tensor* k_pa
   return OJC_OK;
 }
 
+constexpr int MAX_CTAS = 2 * REDUCE_SMS;   // of the tiles kernel: the partition, and so the bits, do not depend on the opened device
+
+// The tiles kernel's workspace: the split units, then (m, l) and outputs of two row tiles (of 64 rows at most) for each CTA.
+uint64_t tiles_workspace(int64_t dim) { return 8192 + (uint64_t)2 * MAX_CTAS * 64 * (dim + 2) * 4; }
+
+// 16-byte rows: base and strides aligned
+bool rows_aligned(const ojc_tensor* t, int axes) {
+  const int64_t per = 16 / (int64_t)dtype_size(t->dtype);
+  if ((uintptr_t)t->data & 15) return false;
+  for (int i = 0; i < axes; ++i) if (t->stride[i] < 0 || t->stride[i] % per) return false;
+  return true;
+}
+
+bool tiles_take(const ojc_tensor* q, const ojc_tensor* k, const ojc_tensor* v, const ojc_tensor* out, int64_t dim) {
+  const bool shape = dim == 64 || dim == 96 || dim == 128 || (q->dtype == OJC_BF16 && (dim == 80 || dim == 256));
+  return shape && rows_aligned(q, 2) && rows_aligned(k, 3) && rows_aligned(v, 3) && rows_aligned(out, 2);
+}
+
+struct AttnCall {
+  ojc_backend* be; const char* op;
+  const ojc_tensor *q, *k, *v; ojc_tensor* out; float* lse;
+  PassIndex ix; AttnDims a; float scale; void* work;
+};
+
+template <class T, int D, int MW>
+ojc_status tiles_launch(const AttnCall& c) {
+  constexpr int smem = TileShape<T, D, MW>::SMEM;
+  static PerDeviceFlag attr;
+  if (!attr[c.be->device]) {
+    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tiles_kernel<T, D, MW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), c.op);
+    attr[c.be->device] = true;
+  }
+  const int ctas = TileShape<T, D, MW>::CTAS_PER_SM * REDUCE_SMS, group = (int)(c.a.heads / c.a.kv_heads);
+  TileWork w;
+  w.split = (SplitUnit*)c.work;
+  w.ml = (float2*)((char*)c.work + 8192);
+  w.o = (float*)(w.ml + (size_t)2 * MAX_CTAS * 64);
+  paged_attention_tiles_kernel<T, D, MW><<<ctas, TILE_WARPS * 32, smem, c.be->stream>>>(rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
+                                                                                       rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, (int)c.a.kv_heads, c.scale, c.be->fault_dev);
+  OJC_LAUNCHED(c.be, c.op);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 16 * MW);
+  cfg.blockDim = dim3(128);
+  cfg.stream = c.be->stream;
+  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T>, c.ix, rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, 16 * MW, D, c.scale, c.be->fault_dev), c.op);
+  OJC_LAUNCHED(c.be, c.op);
+  return OJC_OK;
+}
+
+template <class T, int D>
+ojc_status tiles_by_rows(const AttnCall& c) {
+  // rows of a KV head in a request of average length: what the host knows without a readback
+  const int64_t rows = (c.a.tokens + c.ix.batch - 1) / c.ix.batch * (c.a.heads / c.a.kv_heads);
+  if (rows <= 16) return tiles_launch<T, D, 1>(c);
+  if (rows <= 32) return tiles_launch<T, D, 2>(c);
+  return tiles_launch<T, D, 4>(c);
+}
+
+template <class T>
+ojc_status tiles_by_dim(const AttnCall& c) {
+  if (c.a.dim == 64) return tiles_by_rows<T, 64>(c);
+  if (c.a.dim == 96) return tiles_by_rows<T, 96>(c);
+  if constexpr (std::is_same<T, bf16>::value) {
+    if (c.a.dim == 80) return tiles_by_rows<T, 80>(c);
+    if (c.a.dim == 256) return tiles_by_rows<T, 256>(c);
+  }
+  return tiles_by_rows<T, 128>(c);
+}
+
 }  // namespace
 
 extern "C" {
@@ -142,7 +752,7 @@ ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor
   if (!bytes) return ojc_fail(OJC_ERR_BACKEND, op, "null out pointer");
   AttnDims a;
   OJC_TRY(attn_dims(op, q, k_pages, &a));
-  *bytes = 256;
+  *bytes = tiles_workspace(a.dim);
   return OJC_OK;
 }
 
@@ -190,8 +800,11 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
                      window < 0 ? 0 : window};
   const float scale = 1.0f / sqrtf((float)a.dim);
   float* lse_out = lse ? (float*)lse->data : nullptr;
+  const AttnCall call{be, op, q, k_pages, v_pages, out, lse_out, ix, a, scale, workspace};
+  const bool tiles = tiles_take(q, k_pages, v_pages, out, a.dim);
   return dispatch_float(op, q->dtype, [&](auto t) {
     using T = decltype(t);
+    if (tiles) return tiles_by_dim<T>(call);
     paged_attention_rows_kernel<T><<<(unsigned)((a.tokens * a.heads + 3) / 4), 128, 4 * a.dim * 4, be->stream>>>(
         rows_view<const T>(q), pages_view<const T>(k_pages), pages_view<const T>(v_pages), ix, rows_view<T>(out), lse_out, (int)a.heads, (int)(a.heads / a.kv_heads), (int)a.dim,
         scale, be->fault_dev);
