@@ -63,6 +63,7 @@ class Tensor:
         self.strides = tuple(strides) if strides is not None else _contig_strides(self.shape)
         self._owner = owner  # keeps the storage alive for views
         self._owns = owner is None
+        self._ref = None     # the descriptor as the C ABI takes it, made at the first call
 
     def __del__(self):
         if getattr(self, "_owns", False) and self.ptr and self.backend is not None and self.backend._handle:
@@ -98,7 +99,11 @@ def _dt(choice, default):
 
 
 def _p(t: "Tensor | None"):
-    return C.byref(t.c()) if t is not None else None
+    if t is None:
+        return None
+    if t._ref is None:
+        t._ref = C.byref(t.c())
+    return t._ref
 
 
 @dataclass

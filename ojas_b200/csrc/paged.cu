@@ -1,6 +1,10 @@
 // Decode over a paged KV cache: the plan of a pass (block tables, slots, positions, ancestor masks), rotary positions and the cache write.
 // The attention that reads the pages is paged_attn.cu.
+#include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
 
 #include "dispatch.cuh"
 #include "paged.cuh"
@@ -135,10 +139,160 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   if (bad) raise_fault(fault, OP_PAGED_RANGE);
 }
 
+// ======================================================================== vectors of a head
+// V elements as floats, in loads and stores of at most 16 bytes
+template <int V> __device__ __forceinline__ void load_v(const float* p, float (&v)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) { const float4 x = *reinterpret_cast<const float4*>(p + i); v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w; }
+  } else { const float2 x = *reinterpret_cast<const float2*>(p); v[0] = x.x; v[1] = x.y; }
+}
+template <int V> __device__ __forceinline__ void store_v(float* p, const float (&v)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+}
+template <int V> struct Words;
+template <> struct Words<2> { typedef uint32_t type; };
+template <> struct Words<4> { typedef uint2 type; };
+template <> struct Words<8> { typedef uint4 type; };
+template <int V> __device__ __forceinline__ void load_v(const bf16* p, float (&v)[V]) {
+  union { typename Words<V>::type w; uint32_t u[V / 2]; } x;
+  x.w = *reinterpret_cast<const typename Words<V>::type*>(p);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) { v[2 * i] = __uint_as_float(x.u[i] << 16); v[2 * i + 1] = __uint_as_float(x.u[i] & 0xffff0000u); }
+}
+template <int V> __device__ __forceinline__ void store_v(bf16* p, const float (&v)[V]) {
+  union { typename Words<V>::type w; bf16 b[V]; } x;
+#pragma unroll
+  for (int i = 0; i < V; ++i) x.b[i] = __float2bfloat16_rn(v[i]);
+  *reinterpret_cast<typename Words<V>::type*>(p) = x.w;
+}
+
+// The rotation of one vector's worth of pairs: V pairs (i, i + half) in the half layout, V / 2 neighbours in the interleaved one. What passes
+// through is an item of its own, moved as it is.
+template <int V, bool INTER> struct Turn {
+  static constexpr int PAIRS = INTER ? V / 2 : V;
+  float c[PAIRS], s[PAIRS];
+  __device__ __forceinline__ void set(const ojc_rope& rope, int first_pair, uint32_t position, float sign) {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) { rope_turn(rope.turns[first_pair + i], position, rope.amplitude, &c[i], &s[i]); s[i] *= sign; }
+  }
+  __device__ __forceinline__ void apply(float (&a)[V], float (&b)[V]) const {   // a alone in the interleaved layout
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      float& u = INTER ? a[2 * i] : a[i];
+      float& v = INTER ? a[2 * i + 1] : b[i];
+      const float x = turned_first(u, v, c[i], s[i]);
+      v = turned_second(u, v, c[i], s[i]);
+      u = x;
+    }
+  }
+};
+
+// Rotary positions by vectors: a thread forms its pairs' sines and cosines once and goes through `step` heads with them, HEADS at a time so that their
+// loads are in flight together.
+template <class T, int V, bool INTER>
+__global__ void __launch_bounds__(256)
+rope_vector_kernel(const __grid_constant__ ojc_rope rope, const T* x, T* y, const uint32_t* __restrict__ positions, uint32_t rows, uint32_t time, uint32_t pos_rows, int heads, int step,
+                   int dim, int64_t xb, int64_t xt, int64_t xh, int64_t yb, int64_t yt, int64_t yh, float sign) {
+  constexpr int HEADS = 4;
+  const uint32_t half = rope.rotary_dim / 2, turned = (INTER ? rope.rotary_dim : half) / V, items = turned + (dim - rope.rotary_dim) / V;
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, row = at / items, item = at % items;
+  if (row >= rows) return;
+  const int h0 = blockIdx.y * step, h1 = min(heads, h0 + step);
+  const uint32_t b = row / time, t = row - b * time;
+  const bool turns = item < turned;
+  const int e = turns ? (int)(item * V) : (int)(rope.rotary_dim + (item - turned) * V);
+  x += b * xb + t * xt + e;
+  y += b * yb + t * yt + e;
+  Turn<V, INTER> turn;
+  if (turns) turn.set(rope, INTER ? e / 2 : e, positions[pos_rows == rows ? row : t], sign);
+  for (int h = h0; h < h1; h += HEADS) {
+    float u[HEADS][V], v[HEADS][V];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) if (h + i < h1) {
+      load_v<V>(x + (h + i) * xh, u[i]);
+      if (turns && !INTER) load_v<V>(x + (h + i) * xh + half, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) if (h + i < h1) {
+      if (turns) turn.apply(u[i], v[i]);
+      store_v<V>(y + (h + i) * yh, u[i]);
+      if (turns && !INTER) store_v<V>(y + (h + i) * yh + half, v[i]);
+    }
+  }
+}
+
+// The cache write by vectors: the same items, a rotated key vector (or pair of vectors) with the value's at the same place.
+template <class S, class D, int V, bool INTER>
+__global__ void __launch_bounds__(256)
+paged_kv_write_vector_kernel(const __grid_constant__ ojc_rope rope, PagesView<D> kp, PagesView<D> vp, RowsView<const S> k, RowsView<const S> v, const uint32_t* __restrict__ slots,
+                             const uint32_t* __restrict__ positions, uint32_t tokens, int heads, int step, int dim, uint32_t page, uint32_t n_slots, uint32_t* fault) {
+  constexpr int HEADS = 2;
+  const uint32_t half = rope.rotary_dim / 2, turned = (INTER ? rope.rotary_dim : half) / V, items = turned + (dim - rope.rotary_dim) / V;
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, t = at / items, item = at % items;
+  if (t >= tokens) return;
+  const uint32_t slot = slots[t];
+  if (slot == OJC_NONE) return;
+  if (slot >= n_slots) { if (item == 0) raise_fault(fault, OP_PAGED_RANGE); return; }
+  const uint32_t pg = slot / page, off = slot - pg * page;
+  const int h0 = blockIdx.y * step, h1 = min(heads, h0 + step);
+  const bool turns = item < turned;
+  const int e = turns ? (int)(item * V) : (int)(rope.rotary_dim + (item - turned) * V);
+  const S *sk = k.ptr + t * k.sn + e, *sv = v.ptr + t * v.sn + e;
+  D *dk = kp.ptr + pg * kp.sp + off * kp.st + e, *dv = vp.ptr + pg * vp.sp + off * vp.st + e;
+  Turn<V, INTER> turn;
+  if (turns) turn.set(rope, INTER ? e / 2 : e, positions[t], 1.0f);
+  for (int h = h0; h < h1; h += HEADS) {
+    float a[HEADS][V], b[HEADS][V], c[HEADS][V], d[HEADS][V];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) if (h + i < h1) {
+      load_v<V>(sk + (h + i) * k.sh, a[i]);
+      load_v<V>(sv + (h + i) * v.sh, c[i]);
+      if (turns && !INTER) { load_v<V>(sk + (h + i) * k.sh + half, b[i]); load_v<V>(sv + (h + i) * v.sh + half, d[i]); }
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) if (h + i < h1) {
+      if (turns) turn.apply(a[i], b[i]);
+      store_v<V>(dk + (h + i) * kp.sh, a[i]);
+      store_v<V>(dv + (h + i) * vp.sh, c[i]);
+      if (turns && !INTER) { store_v<V>(dk + (h + i) * kp.sh + half, b[i]); store_v<V>(dv + (h + i) * vp.sh + half, d[i]); }
+    }
+  }
+}
+
+// The widest vector (8, 4 or 2 elements, at most 16 bytes of the narrower type's) that the rotated part's pieces, the rest and every row start allow; 0: none
+int vector_of(int layout, int rotary, int64_t dim, std::initializer_list<std::pair<const ojc_tensor*, int>> tensors) {
+  for (int v = 8; v >= 2; v /= 2) {
+    bool fits = dim % v == 0 && (layout ? rotary : rotary / 2) % v == 0;
+    for (auto& [t, axes] : tensors) {
+      const int64_t size = (int64_t)dtype_size(t->dtype), bytes = std::min<int64_t>(16, v * size);
+      fits = fits && (uintptr_t)t->data % bytes == 0;
+      for (int i = 0; i < axes; ++i) fits = fits && t->stride[i] * size % bytes == 0;
+    }
+    if (fits) return v;
+  }
+  return 0;
+}
+
+// How many heads a thread goes through: all of them when the items alone fill the GPU twice over, fewer when there are few
+int heads_per_thread(const ojc_backend* be, int64_t items, int64_t heads) {
+  return (int)std::max<int64_t>(1, std::min(heads, items * heads / ((int64_t)be->sm_count * 2048)));
+}
+
+template <class F> ojc_status by_vector(int v, int layout, F&& f) {
+  auto with = [&](auto n) { return layout ? f(n, std::true_type()) : f(n, std::false_type()); };
+  if (v == 8) return with(std::integral_constant<int, 8>());
+  if (v == 4) return with(std::integral_constant<int, 4>());
+  return with(std::integral_constant<int, 2>());
+}
+
 // ======================================================================== rotary positions
-// One thread per pair of a (token, head), and one per element behind the rotated part.
+// Any alignment: one thread per pair of a (token, head), and one per element behind the rotated part.
 template <class T>
-__global__ void rope_kernel(const __grid_constant__ ojc_rope rope, const T* __restrict__ x, T* __restrict__ y, const uint32_t* __restrict__ positions, int64_t rows, int64_t time,
+__global__ void rope_kernel(const __grid_constant__ ojc_rope rope, const T* x, T* y, const uint32_t* __restrict__ positions, int64_t rows, int64_t time,
                             int64_t pos_rows, int heads, int dim, int64_t xb, int64_t xt, int64_t xh, int64_t yb, int64_t yt, int64_t yh, float sign) {
   const int half = rope.rotary_dim / 2, items = half + dim - rope.rotary_dim;
   const int64_t total = rows * heads * items;
@@ -153,8 +307,8 @@ __global__ void rope_kernel(const __grid_constant__ ojc_rope rope, const T* __re
     s *= sign;
     const int i0 = rope.layout ? 2 * e : e, i1 = rope.layout ? 2 * e + 1 : e + half;
     const float u = ldf(px, i0), v = ldf(px, i1);
-    stf(py, i0, u * c - v * s);
-    stf(py, i1, v * c + u * s);
+    stf(py, i0, turned_first(u, v, c, s));
+    stf(py, i1, turned_second(u, v, c, s));
   }
 }
 
@@ -181,7 +335,7 @@ __global__ void paged_kv_write_kernel(const __grid_constant__ ojc_rope rope, boo
       const float other = ldf(pk, rope.layout ? e ^ 1 : second ? e - half : e + half);
       float c, s;
       rope_turn(rope.turns[pair], positions[t], rope.amplitude, &c, &s);
-      a = second ? a * c + other * s : a * c - other * s;
+      a = second ? turned_second(other, a, c, s) : turned_first(a, other, c, s);
     }
     stf(kp.ptr + pg * kp.sp + off * kp.st + h * kp.sh, e, a);
     stf(vp.ptr + pg * vp.sp + off * vp.st + h * vp.sh, e, ldf(v.ptr + t * v.sn + h * v.sh, e));
@@ -213,6 +367,18 @@ ojc_status rope_run(ojc_backend* be, const char* op, const ojc_rope* rope, const
   const int64_t xb = r == 4 ? x->stride[0] : 0, yb = r == 4 ? y->stride[0] : 0;
   return dispatch_float(op, x->dtype, [&](auto t) {
     using T = decltype(t);
+    const int v = vector_of(rope->layout, rope->rotary_dim, dim, {{x, r - 1}, {y, r - 1}});
+    if (v && rows * dim < INT32_MAX) {
+      const int64_t per_row = ((rope->layout ? rope->rotary_dim : rope->rotary_dim / 2) + dim - rope->rotary_dim) / v, step = heads_per_thread(be, rows * per_row, heads);
+      const dim3 grid((unsigned)((rows * per_row + 255) / 256), (unsigned)((heads + step - 1) / step));
+      if (grid.y <= 65535) return by_vector(v, rope->layout, [&](auto n, auto inter) {
+        rope_vector_kernel<T, decltype(n)::value, decltype(inter)::value><<<grid, 256, 0, be->stream>>>(
+            *rope, (const T*)x->data, (T*)y->data, (const uint32_t*)positions->data, (uint32_t)rows, (uint32_t)time, (uint32_t)np, (int)heads, (int)step, (int)dim, xb,
+            x->stride[r - 3], x->stride[r - 2], yb, y->stride[r - 3], y->stride[r - 2], sign);
+        OJC_LAUNCHED(be, op);
+        return OJC_OK;
+      });
+    }
     const int64_t items = rows * heads * (dim - rope->rotary_dim / 2);
     rope_kernel<T><<<elementwise_grid(be, items, 256), 256, 0, be->stream>>>(*rope, (const T*)x->data, (T*)y->data, (const uint32_t*)positions->data, rows, time, np, (int)heads,
                                                                              (int)dim, xb, x->stride[r - 3], x->stride[r - 2], yb, y->stride[r - 3], y->stride[r - 2], sign);
@@ -336,8 +502,21 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
     using S = decltype(s);
     return dispatch_float(op, k_pages->dtype, [&](auto d) {
       using D = decltype(d);
+      ojc_rope turn = rope ? *rope : ojc_rope{};
+      const int vec = vector_of(turn.layout, turn.rotary_dim, dim, {{k_pages, 3}, {v_pages, 3}, {k, 2}, {v, 2}});
+      if (vec && tokens * dim < INT32_MAX) {
+        const int64_t per_row = ((turn.layout ? turn.rotary_dim : turn.rotary_dim / 2) + dim - turn.rotary_dim) / vec, step = heads_per_thread(be, tokens * per_row, heads);
+        const dim3 grid((unsigned)((tokens * per_row + 255) / 256), (unsigned)((heads + step - 1) / step));
+        if (grid.y <= 65535) return by_vector(vec, turn.layout, [&](auto n, auto inter) {
+          paged_kv_write_vector_kernel<S, D, decltype(n)::value, decltype(inter)::value><<<grid, 256, 0, be->stream>>>(
+              turn, pages_view<D>(k_pages), pages_view<D>(v_pages), rows_view<const S>(k), rows_view<const S>(v), (const uint32_t*)slots->data,
+              rope ? (const uint32_t*)positions->data : nullptr, (uint32_t)tokens, (int)heads, (int)step, (int)dim, (uint32_t)page, (uint32_t)(pages * page), be->fault_dev);
+          OJC_LAUNCHED(be, op);
+          return OJC_OK;
+        });
+      }
       paged_kv_write_kernel<S, D><<<elementwise_grid(be, numel(k), 256), 256, 0, be->stream>>>(
-          rope ? *rope : ojc_rope{}, rope != nullptr, pages_view<D>(k_pages), pages_view<D>(v_pages), rows_view<const S>(k), rows_view<const S>(v), (const uint32_t*)slots->data,
+          turn, rope != nullptr, pages_view<D>(k_pages), pages_view<D>(v_pages), rows_view<const S>(k), rows_view<const S>(v), (const uint32_t*)slots->data,
           rope ? (const uint32_t*)positions->data : nullptr, tokens, (int)heads, (int)dim, (uint32_t)page, pages * page, be->fault_dev);
       OJC_LAUNCHED(be, op);
       return OJC_OK;

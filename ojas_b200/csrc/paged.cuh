@@ -26,9 +26,12 @@ inline RowsView<P> rows_view(const ojc_tensor* t) { return RowsView<P>{(P*)t->da
 __device__ __forceinline__ void rope_turn(uint64_t turns, uint32_t position, float amplitude, float* c, float* s) {
   const uint64_t t = turns * position;
   sincospif((float)(int32_t)(uint32_t)(t >> 32) * 4.656612873077393e-10f, s, c);
-  *c *= amplitude;
-  *s *= amplitude;
+  *c = __fmul_rn(*c, amplitude);
+  *s = __fmul_rn(*s, amplitude);
 }
+// (u, v) turned: one product rounded, then a fused multiply-add, spelled out so that every kernel gives the same bits
+__device__ __forceinline__ float turned_first(float u, float v, float c, float s) { return __fmaf_rn(u, c, -__fmul_rn(v, s)); }
+__device__ __forceinline__ float turned_second(float u, float v, float c, float s) { return __fmaf_rn(v, c, __fmul_rn(u, s)); }
 #endif
 
 ojc_status rope_check(const char* op, const ojc_rope* rope, int64_t head_dim);
