@@ -16,6 +16,7 @@ struct PassIndex {       // the pass's index tables (all U32)
   int batch, words;
   int64_t tokens, width, pages;
   uint32_t page;
+  int page_shift;        // log2 of the page, or -1
   int64_t window;        // 0: none
 };
 
@@ -127,9 +128,7 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 constexpr int BLOCK_KEYS = 64, TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {   // zeros when the source is not there
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t a) {
@@ -160,32 +159,33 @@ __device__ __forceinline__ float quad_sum(float v) { v += __shfl_xor_sync(0xffff
 struct SplitUnit { int pieces, request, kv_head, row_tile; };
 struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][16 MW][D], ml [2 CTAs][16 MW], split [CTAs]
 
-struct Request { int64_t cached; uint32_t first; int fresh, first_block, blocks, row_tiles; };
+struct Request { uint32_t cached, first; int fresh, first_block, blocks, row_tiles; };
 __device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int group, int tile_rows, bool* bad) {
   Request r;
-  const uint32_t first = ix.starts[b], end = ix.starts[b + 1];
-  r.cached = ix.cached[b];
-  r.first = first;
-  const bool wrong = end < first || end > ix.tokens || r.cached + (int64_t)(end - first) > ix.width * ix.page;
+  const uint32_t first = ix.starts[b], end = ix.starts[b + 1], cached = ix.cached[b];
+  const bool wrong = end < first || end > ix.tokens || (int64_t)cached + (int64_t)(end - first) > ix.width * ix.page;
   *bad |= wrong;
+  r.cached = wrong ? 0 : cached;
+  r.first = first;
   r.fresh = wrong ? 0 : (int)(end - first);
-  const int64_t from = ix.window > 0 ? max((int64_t)0, r.cached - ix.window + 1) : 0;   // positions of new tokens are at least `cached`
-  r.first_block = (int)(from / BLOCK_KEYS);
-  r.blocks = (int)((r.cached + r.fresh + BLOCK_KEYS - 1) / BLOCK_KEYS) - r.first_block;
-  r.row_tiles = (r.fresh * group + tile_rows - 1) / tile_rows;
-  if (r.fresh == 0) r.blocks = 0;
+  const int64_t from = ix.window > 0 ? (int64_t)r.cached - ix.window + 1 : 0;   // positions of new tokens are at least `cached`
+  r.first_block = from > 0 ? (int)(from / BLOCK_KEYS) : 0;
+  r.blocks = r.fresh == 0 ? 0 : (int)((r.cached + (uint32_t)r.fresh + BLOCK_KEYS - 1) / BLOCK_KEYS) - r.first_block;
+  r.row_tiles = (int)((uint32_t)(r.fresh * group + tile_rows - 1) / (uint32_t)tile_rows);
   return r;
 }
 
 // A place on the line of work; all threads of a CTA hold the same one.
 struct Cursor {
   Request r;
-  int b, unit, block;     // unit: kv_head * row_tiles + row_tile; block counts from 0
+  int b, hk, row_tile, block;     // block counts from 0
   __device__ __forceinline__ void step(const PassIndex& ix, int group, int tile_rows, int kv_heads, bool* bad) {
     if (++block < r.blocks) return;
     block = 0;
-    if (++unit < kv_heads * r.row_tiles) return;
-    unit = 0;
+    if (++row_tile < r.row_tiles) return;
+    row_tile = 0;
+    if (++hk < kv_heads) return;
+    hk = 0;
     do { if (++b >= ix.batch) return; r = load_request(ix, b, group, tile_rows, bad); } while (r.blocks == 0);
   }
 };
@@ -212,8 +212,8 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   constexpr int KSTEP = F32 ? 8 : 16, KSTEPS = D / KSTEP;
   extern __shared__ __align__(128) uint8_t raw[];
   float* joint = reinterpret_cast<float*>(raw + STAGES * S::STAGE);                                   // [16][D] and [16] (m, l): the warps' outputs meet here
-  int64_t* offsets = reinterpret_cast<int64_t*>(raw + STAGES * S::STAGE + S::JOINT);
-  T* q_tile = reinterpret_cast<T*>(offsets + TILE_WARPS * 32);                                          // only without Q_IN_REGS
+  uint64_t* rows_at = reinterpret_cast<uint64_t*>(raw + STAGES * S::STAGE + S::JOINT);
+  T* q_tile = reinterpret_cast<T*>(rows_at + TILE_WARPS * 32);                                          // only without Q_IN_REGS
   __shared__ unsigned long long s_sum[TILE_WARPS], s_at;
   __shared__ int s_b;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
@@ -253,44 +253,55 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   Cursor use;
   use.b = s_b;
   use.r = load_request(ix, use.b, group, TILE_ROWS, &bad);
-  use.unit = (int)((begin - s_at) / (unsigned)use.r.blocks);
-  use.block = (int)((begin - s_at) % (unsigned)use.r.blocks);
+  {
+    const uint32_t unit = (uint32_t)((begin - s_at) / (unsigned)use.r.blocks);
+    use.block = (int)(begin - s_at - (unsigned long long)unit * (unsigned)use.r.blocks);
+    use.hk = (int)(unit / (unsigned)use.r.row_tiles);
+    use.row_tile = (int)(unit % (unsigned)use.r.row_tiles);
+  }
   Cursor ahead = use;                                                                                   // the block whose pages are looked up next
-  const int64_t todo = (int64_t)(end - begin);
+  const int todo = (int)(end - begin);
 
-  // ---- copies: warp w fetches keys 16 w .. 16 w + 15 of a block; lane l < 16 looks up key l's place
+  // ---- copies: warp w fetches keys 16 w .. 16 w + 15 of a block; lane l looks up key l's row of K, lane 16 + l its row of V. Places behind the last
+  // one repeat it: what lies there is masked like any place that is not seen.
+  const PagesView<const T>& mine = lane < 16 ? kp : vp;
+  const char* const mine_ptr = (const char*)mine.ptr;
+  const int64_t mine_sp = mine.sp * (int)sizeof(T), mine_st = mine.st * (int)sizeof(T), mine_sh = mine.sh * (int)sizeof(T);
   uint32_t id = 0, off = 0;
   int hk_ahead = 0;
-  bool there = false;
   auto look_up = [&]() {
-    const int64_t j = (int64_t)(ahead.r.first_block + ahead.block) * BLOCK_KEYS + 16 * warp + (lane & 15);
-    there = j < ahead.r.cached + ahead.r.fresh;
-    hk_ahead = ahead.unit / ahead.r.row_tiles;
-    if (there) {
-      const uint32_t pi = (uint32_t)j / ix.page;
-      off = (uint32_t)j - pi * ix.page;
-      id = ix.tables[(int64_t)ahead.b * ix.width + pi];
-    }
+    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + 16 * warp + (lane & 15)), last);
+    const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
+    off = j - pi * ix.page;
+    id = ix.tables[(int64_t)ahead.b * ix.width + pi];
+    hk_ahead = ahead.hk;
     ahead.step(ix, group, TILE_ROWS, kv_heads, &bad);
   };
-  int64_t* my_offsets = offsets + warp * 32;
+  uint64_t* my_rows = rows_at + warp * 32;
+  const uint32_t k_base = smem_addr(raw) + (16 * warp + lane / CHUNKS) * S::K_PITCH * (int)sizeof(T) + (lane % CHUNKS) * 16;
+  const uint32_t v_base = smem_addr(raw) + (BLOCK_KEYS * S::K_PITCH + (16 * warp + lane / CHUNKS) * S::V_PITCH) * (int)sizeof(T) + (lane % CHUNKS) * 16;
   auto copy_block = [&](int stage) {
-    if (there && id >= ix.pages) { bad = true; there = false; }
-    my_offsets[lane] = !there ? -1 : lane < 16 ? id * kp.sp + off * kp.st + hk_ahead * kp.sh : id * vp.sp + off * vp.st + hk_ahead * vp.sh;
+    if (id >= ix.pages) { bad = true; id = 0; }
+    my_rows[lane] = (uint64_t)(mine_ptr + (int64_t)id * mine_sp + (int64_t)off * mine_st + (int64_t)hk_ahead * mine_sh);
     __syncwarp();
-    const uint32_t base = smem_addr(raw) + stage * S::STAGE + (16 * warp) * S::K_PITCH * (int)sizeof(T);
-    const uint32_t vbase = smem_addr(raw) + stage * S::STAGE + (BLOCK_KEYS * S::K_PITCH + 16 * warp * S::V_PITCH) * (int)sizeof(T);
+    const uint32_t ka = k_base + stage * S::STAGE, va = v_base + stage * S::STAGE;
+    if constexpr (32 % CHUNKS == 0) {                                                                   // a lane keeps its column of 16 bytes
+      constexpr int ROWS = 32 / CHUNKS;
+      const uint64_t* at = my_rows + lane / CHUNKS;
+      const int c = (lane % CHUNKS) * 16;
 #pragma unroll
-    for (int i = 0; i < CHUNKS / 2; ++i) {
-      const int at = lane + 32 * i, row = at / CHUNKS, c = at % CHUNKS;
-      const int64_t ko = my_offsets[row];
-      copy16(base + row * S::K_PITCH * (int)sizeof(T) + c * 16, kp.ptr + (ko < 0 ? 0 : ko) + c * PER, ko >= 0);
-    }
+      for (int i = 0; i < 16 / ROWS; ++i) copy16(ka + i * ROWS * S::K_PITCH * (int)sizeof(T), (const char*)at[i * ROWS] + c);
 #pragma unroll
-    for (int i = 0; i < CHUNKS / 2; ++i) {
-      const int at = lane + 32 * i, row = at / CHUNKS, c = at % CHUNKS;
-      const int64_t vo = my_offsets[16 + row];
-      copy16(vbase + row * S::V_PITCH * (int)sizeof(T) + c * 16, vp.ptr + (vo < 0 ? 0 : vo) + c * PER, vo >= 0);
+      for (int i = 0; i < 16 / ROWS; ++i) copy16(va + i * ROWS * S::V_PITCH * (int)sizeof(T), (const char*)at[16 + i * ROWS] + c);
+    } else {
+      const uint32_t kw0 = smem_addr(raw) + stage * S::STAGE + 16 * warp * S::K_PITCH * (int)sizeof(T);
+      const uint32_t vw0 = smem_addr(raw) + stage * S::STAGE + (BLOCK_KEYS * S::K_PITCH + 16 * warp * S::V_PITCH) * (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < CHUNKS / 2; ++i) {
+        const int n = lane + 32 * i, row = n / CHUNKS, c = n % CHUNKS * 16;
+        copy16(kw0 + row * S::K_PITCH * (int)sizeof(T) + c, (const char*)my_rows[row] + c);
+        copy16(vw0 + row * S::V_PITCH * (int)sizeof(T) + c, (const char*)my_rows[16 + row] + c);
+      }
     }
     __syncwarp();
   };
@@ -304,27 +315,28 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   uint32_t qf[S::Q_IN_REGS ? KSTEPS : 1][4];
   float o[OT][4], m[2], l[2];
   bool any[2];
-  int64_t low[2], low_most = -1;
+  uint32_t from[2], from_most = 0;                                                                      // the first position in a row's window
   int local[2];
   bool live[2];
   const float c2 = scale * 1.4426950408889634f;
   unsigned long long piece_begin = begin;
 
-  for (int64_t f = 0; f < todo; ++f) {
-    const int row_tile = use.unit % use.r.row_tiles, hk = use.unit / use.r.row_tiles;
+  int stage = 0;
+  for (int f = 0; f < todo; ++f) {
+    const int row_tile = use.row_tile, hk = use.hk;
     if (f == 0 || use.block == 0) {                                                                     // a new unit: its rows
       piece_begin = begin + f;
-      low_most = -1;
+      from_most = 0;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = row_tile * TILE_ROWS + 16 * mw + quad + 8 * x;
         live[x] = r < use.r.fresh * group;
         local[x] = live[x] ? r / group : 0;
         const int64_t t = use.r.first + local[x];
-        const int64_t place = ix.positions ? (int64_t)ix.positions[t] : use.r.cached + local[x];
-        low[x] = ix.window > 0 ? place - ix.window : -1;
+        const uint32_t place = ix.positions ? ix.positions[t] : use.r.cached + (uint32_t)local[x];
+        from[x] = ix.window > 0 && place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
         if (live[x] && ix.window > 0 && place < use.r.cached) bad = true;
-        if (live[x]) low_most = max(low_most, low[x]);
+        if (live[x]) from_most = max(from_most, from[x]);
         m[x] = -INFINITY; l[x] = 0.0f; any[x] = false;
         if (S::Q_IN_REGS) {
           const uint32_t* p = reinterpret_cast<const uint32_t*>(q.ptr + t * q.sn + (int64_t)(hk * group + (live[x] ? r % group : 0)) * q.sh);
@@ -332,7 +344,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
           for (int k = 0; k < KSTEPS; ++k) { qf[k][x] = live[x] ? p[8 * k + pair] : 0u; qf[k][2 + x] = live[x] ? p[8 * k + 4 + pair] : 0u; }
         }
       }
-      if (ix.window > 0) for (int s = 16; s > 0; s >>= 1) low_most = max(low_most, __shfl_xor_sync(0xffffffffu, low_most, s));
+      if (ix.window > 0) from_most = __reduce_max_sync(0xffffffffu, from_most);
       if (!S::Q_IN_REGS) {
         __syncthreads();
         for (int i = tid; i < TILE_ROWS * CHUNKS; i += TILE_WARPS * 32) {
@@ -352,14 +364,14 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     copies_wait<STAGES - 2>();
     if (MW == 1) __syncwarp(); else __syncthreads();
     {                                                                                                   // the stage that the last block left
-      const int64_t next = f + STAGES - 1;
-      if (next < todo) { copy_block((int)(next % STAGES)); if (next + 1 < todo) look_up(); }
+      const int next = f + STAGES - 1;
+      if (next < todo) { copy_block(stage == 0 ? STAGES - 1 : stage - 1); if (next + 1 < todo) look_up(); }
       copies_commit();
     }
-    const int stage = (int)(f % STAGES);
     const T* kt = reinterpret_cast<const T*>(raw + stage * S::STAGE) + kw * KEYS * S::K_PITCH;
     const T* vt = reinterpret_cast<const T*>(raw + stage * S::STAGE) + BLOCK_KEYS * S::K_PITCH + kw * KEYS * S::V_PITCH;
-    const int64_t j0 = (int64_t)(use.r.first_block + use.block) * BLOCK_KEYS + kw * KEYS;
+    const uint32_t j0 = (uint32_t)((use.r.first_block + use.block) * BLOCK_KEYS + kw * KEYS);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
 
     float s[NT][4];
 #pragma unroll
@@ -402,21 +414,21 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     // ---- what the rows see: everything in a block below the cached length and inside every row's window
     uint32_t sees = 0xffffffffu;                                                                        // bit 4 n + element
     bool poisoned = false;
-    if (j0 + KEYS > use.r.cached || (ix.window > 0 && j0 <= low_most)) {
+    if (j0 + KEYS > use.r.cached || j0 < from_most) {
       sees = 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int x = e >> 1;
-          const int64_t j = j0 + 8 * n + 2 * pair + (e & 1);
+          const uint32_t j = j0 + 8 * n + 2 * pair + (e & 1);
           bool v = live[x];
-          if (j < use.r.cached) v = v && j > low[x];
+          if (j < use.r.cached) v = v && j >= from[x];
           else {
-            const uint32_t d = (uint32_t)(j - use.r.cached);
+            const uint32_t d = j - use.r.cached;
             v = v && d < (uint32_t)use.r.fresh;
             if (v) v = ix.masks ? (d >> 5) < (uint32_t)ix.words && (ix.masks[(int64_t)(use.r.first + local[x]) * ix.words + (d >> 5)] >> (d & 31) & 1u) : d <= (uint32_t)local[x];
-            if (v && ix.window > 0) v = (ix.positions ? (int64_t)ix.positions[use.r.first + d] : j) > low[x];
+            if (v && ix.window > 0) v = (ix.positions ? ix.positions[use.r.first + d] : j) >= from[x];
           }
           if (v) sees |= 1u << (4 * n + e); else s[n][e] = -INFINITY;
         }
@@ -557,7 +569,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
           }
         }
       }
-      const unsigned long long unit_begin = begin + f - use.block;                                      // wraps below zero never: a unit's blocks are on the line
+      const unsigned long long unit_begin = begin + f - use.block;
       const bool whole = unit_done && piece_begin == unit_begin;
       if (kw == 0) {
         const int slot = 2 * blockIdx.x + (piece_begin == unit_begin ? 1 : 0);
@@ -797,7 +809,7 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
   }
   const PassIndex ix{(const uint32_t*)block_tables->data, (const uint32_t*)cached_lens->data, (const uint32_t*)starts->data, masks ? (const uint32_t*)masks->data : nullptr,
                      positions ? (const uint32_t*)positions->data : nullptr, (int)batch, masks ? (int)masks->shape[1] : 0, a.tokens, width, a.pages, (uint32_t)a.page,
-                     window < 0 ? 0 : window};
+                     (a.page & (a.page - 1)) ? -1 : __builtin_ctzll((unsigned long long)a.page), window < 0 ? 0 : window};
   const float scale = 1.0f / sqrtf((float)a.dim);
   float* lse_out = lse ? (float*)lse->data : nullptr;
   const AttnCall call{be, op, q, k_pages, v_pages, out, lse_out, ix, a, scale, workspace};
