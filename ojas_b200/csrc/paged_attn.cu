@@ -2,6 +2,7 @@
 //
 // out_i = sum_j p_ij v_j, p_ij = exp(s_ij - max_j s_ij) / sum, s_ij = q_i . k_j / sqrt(D) over the places j that row i sees: the cached ones inside
 // its window, and of its request's new tokens those in its ancestor mask (or up to itself). One pass over the keys with a running maximum and sum.
+#include <algorithm>
 #include <type_traits>
 
 #include "dispatch.cuh"
@@ -125,6 +126,10 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
 // Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
+#ifndef SHARE_FINER
+#define SHARE_FINER 1
+#define SHARE_LONG 24
+#endif
 constexpr int BLOCK_KEYS = 64, TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -200,10 +205,19 @@ template <class T, int D, int MW> struct TileShape {
   static constexpr int CTAS_PER_SM = SMEM <= 112 * 1024 + 512 ? 2 : 1;
 };
 
+// Shares of the line of work: at least two blocks each up to one wave of CTAs (`wave`: what the GPU holds at once); beyond that up to FINER waves of
+// shares of at least LONG_SHARE blocks, since SMs do not stream equally fast and the later waves go to those that are done.
+constexpr uint32_t FINER = SHARE_FINER, LONG_SHARE = SHARE_LONG;
+__host__ __device__ __forceinline__ uint32_t tile_shares(unsigned long long blocks, uint32_t wave) {
+  const unsigned long long few = (blocks + 1) / 2, many = blocks / LONG_SHARE;
+  const unsigned long long n = few < wave ? few : many < wave ? wave : many;
+  return (uint32_t)(n < (unsigned long long)FINER * wave ? n : (unsigned long long)FINER * wave);
+}
+
 template <class T, int D, int MW>
 __global__ void __launch_bounds__(TILE_WARPS * 32, TileShape<T, D, MW>::CTAS_PER_SM)
 paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesView<const T> vp, PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads,
-                             int group, int kv_heads, float scale, uint32_t* fault) {
+                             int group, int kv_heads, int wave, float scale, uint32_t* fault) {
   using S = TileShape<T, D, MW>;
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr int STAGES = S::STAGES;
@@ -214,50 +228,76 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   float* joint = reinterpret_cast<float*>(raw + STAGES * S::STAGE);                                   // [16][D] and [16] (m, l): the warps' outputs meet here
   uint64_t* rows_at = reinterpret_cast<uint64_t*>(raw + STAGES * S::STAGE + S::JOINT);
   T* q_tile = reinterpret_cast<T*>(rows_at + TILE_WARPS * 32);                                          // only without Q_IN_REGS
-  __shared__ unsigned long long s_sum[TILE_WARPS], s_at;
+  __shared__ uint32_t s_sum[TILE_WARPS], s_at;
   __shared__ int s_b;
+  __shared__ Request s_r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
   bool bad = false, wrong = false;
 
-  // ---- this CTA's stretch [begin, end) of the line of work
-  unsigned long long total = 0;
-  for (int b = tid; b < ix.batch; b += TILE_WARPS * 32) {
-    const Request r = load_request(ix, b, group, TILE_ROWS, &bad);
-    total += (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- this CTA's stretch [begin, end) of the line of work: the blocks in all, an equal share of them, and the request in which the share begins
+  auto blocks_of = [&](const Request& r) {
+    const unsigned long long n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
+    bad |= n >= 1ull << 31;
+    return n >= 1ull << 31 ? 0u : (uint32_t)n;
+  };
+  auto scan = [&](uint32_t n, uint32_t* before) {                                                        // of a chunk of 128 requests; the sum comes back
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const uint32_t a = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += a; }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = n;
+    __syncthreads();
+    *before = n;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < TILE_WARPS; ++w) { if (w < warp) *before += s_sum[w]; sum += s_sum[w]; }
+    return sum;
+  };
+  Request mine_r = {};
+  uint32_t mine_n = 0, mine_at = 0, total = 0;
+  for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {
+    mine_r = {};
+    mine_n = 0;
+    if (b0 + tid < ix.batch) { mine_r = load_request(ix, b0 + tid, group, TILE_ROWS, &bad); mine_n = blocks_of(mine_r); }
+    const uint32_t sum = scan(mine_n, &mine_at);
+    bad |= total + sum < total || total + sum >= 1u << 31;
+    total = bad && (total + sum < total || total + sum >= 1u << 31) ? total : total + sum;
   }
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
-  __syncthreads();
-  total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const unsigned long long ctas = min((unsigned long long)gridDim.x, (total + 1) / 2);                  // at least two blocks each
+  const uint32_t ctas = min(gridDim.x, tile_shares(total, wave));
   if (tid == 0) work.split[blockIdx.x] = SplitUnit{0, 0, 0, 0};
   if (bad) raise_fault(fault, OP_PAGED_RANGE);
   if (blockIdx.x >= ctas) return;
-  const unsigned long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-  unsigned long long carry = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {                                              // the request that holds `begin`
-    const int b = b0 + tid;
-    unsigned long long n = 0;
-    if (b < ix.batch) { const Request r = load_request(ix, b, group, TILE_ROWS, &bad); n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads); }
-    unsigned long long sum = n;
-    for (int o = 1; o < 32; o <<= 1) { const unsigned long long a = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += a; }
-    if (lane == 31) s_sum[warp] = sum;
+  const uint32_t share = total / ctas, longer = total - share * ctas;                                    // the first `longer` shares have one block more
+  auto share_begin = [&](uint32_t c) { return c * share + min(c, longer); };
+  auto share_of = [&](uint32_t block) { return block < longer * (share + 1) ? block / (share + 1) : longer + (block - longer * (share + 1)) / share; };
+  const uint32_t begin = share_begin(blockIdx.x), end = share_begin(blockIdx.x + 1);
+  if (ix.batch <= TILE_WARPS * 32) {
+    mine_at -= mine_n;
+    if (mine_n && mine_at <= begin && begin - mine_at < mine_n) { s_b = tid; s_at = mine_at; s_r = mine_r; }
     __syncthreads();
-    unsigned long long at = carry + sum - n;
-    for (int w = 0; w < TILE_WARPS; ++w) { if (w < warp) at += s_sum[w]; carry += s_sum[w]; }
-    if (n && at <= begin && begin < at + n) { s_b = b; s_at = at; }
-    __syncthreads();
-    if (carry > begin) break;
+  } else {
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {
+      uint32_t n = 0, at;
+      Request r = {};
+      if (b0 + tid < ix.batch) { r = load_request(ix, b0 + tid, group, TILE_ROWS, &bad); n = blocks_of(r); }
+      const uint32_t sum = scan(n, &at);
+      at += carry - n;
+      if (n && at <= begin && begin - at < n) { s_b = b0 + tid; s_at = at; s_r = r; }
+      __syncthreads();
+      carry += sum;
+      if (carry > begin) break;
+    }
   }
   Cursor use;
   use.b = s_b;
-  use.r = load_request(ix, use.b, group, TILE_ROWS, &bad);
+  use.r = s_r;
   {
-    const uint32_t unit = (uint32_t)((begin - s_at) / (unsigned)use.r.blocks);
-    use.block = (int)(begin - s_at - (unsigned long long)unit * (unsigned)use.r.blocks);
-    use.hk = (int)(unit / (unsigned)use.r.row_tiles);
-    use.row_tile = (int)(unit % (unsigned)use.r.row_tiles);
+    const uint32_t unit = (begin - s_at) / (uint32_t)use.r.blocks;
+    use.block = (int)(begin - s_at - unit * (uint32_t)use.r.blocks);
+    use.hk = (int)(unit / (uint32_t)use.r.row_tiles);
+    use.row_tile = (int)(unit - (uint32_t)use.hk * (uint32_t)use.r.row_tiles);
   }
   Cursor ahead = use;                                                                                   // the block whose pages are looked up next
   const int todo = (int)(end - begin);
@@ -267,22 +307,23 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   const PagesView<const T>& mine = lane < 16 ? kp : vp;
   const char* const mine_ptr = (const char*)mine.ptr;
   const int64_t mine_sp = mine.sp * (int)sizeof(T), mine_st = mine.st * (int)sizeof(T), mine_sh = mine.sh * (int)sizeof(T);
-  uint32_t id = 0, off = 0;
-  int hk_ahead = 0;
+  struct Place { uint32_t id, off; int hk; };
   auto look_up = [&]() {
+    Place p;
     const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + 16 * warp + (lane & 15)), last);
     const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
-    off = j - pi * ix.page;
-    id = ix.tables[(int64_t)ahead.b * ix.width + pi];
-    hk_ahead = ahead.hk;
+    p.off = j - pi * ix.page;
+    p.id = ix.tables[(int64_t)ahead.b * ix.width + pi];
+    p.hk = ahead.hk;
     ahead.step(ix, group, TILE_ROWS, kv_heads, &bad);
+    return p;
   };
   uint64_t* my_rows = rows_at + warp * 32;
   const uint32_t k_base = smem_addr(raw) + (16 * warp + lane / CHUNKS) * S::K_PITCH * (int)sizeof(T) + (lane % CHUNKS) * 16;
   const uint32_t v_base = smem_addr(raw) + (BLOCK_KEYS * S::K_PITCH + (16 * warp + lane / CHUNKS) * S::V_PITCH) * (int)sizeof(T) + (lane % CHUNKS) * 16;
-  auto copy_block = [&](int stage) {
-    if (id >= ix.pages) { bad = true; id = 0; }
-    my_rows[lane] = (uint64_t)(mine_ptr + (int64_t)id * mine_sp + (int64_t)off * mine_st + (int64_t)hk_ahead * mine_sh);
+  auto copy_block = [&](int stage, Place p) {
+    if (p.id >= ix.pages) { bad = true; p.id = 0; }
+    my_rows[lane] = (uint64_t)(mine_ptr + (int64_t)p.id * mine_sp + (int64_t)p.off * mine_st + (int64_t)p.hk * mine_sh);
     __syncwarp();
     const uint32_t ka = k_base + stage * S::STAGE, va = v_base + stage * S::STAGE;
     if constexpr (32 % CHUNKS == 0) {                                                                   // a lane keeps its column of 16 bytes
@@ -305,13 +346,6 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     }
     __syncwarp();
   };
-  look_up();
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (s < todo) { copy_block(s); if (s + 1 < todo) look_up(); }
-    copies_commit();
-  }
-
   uint32_t qf[S::Q_IN_REGS ? KSTEPS : 1][4];
   float o[OT][4], m[2], l[2];
   bool any[2];
@@ -319,53 +353,68 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   int local[2];
   bool live[2];
   const float c2 = scale * 1.4426950408889634f;
-  unsigned long long piece_begin = begin;
+  uint32_t piece_begin = begin;
+  Place next_place;
+  auto begin_unit = [&](uint32_t at) {                                                                   // a new unit: its rows
+    const int row_tile = use.row_tile, hk = use.hk;
+    piece_begin = at;
+    from_most = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = row_tile * TILE_ROWS + 16 * mw + quad + 8 * x;
+      live[x] = r < use.r.fresh * group;
+      local[x] = live[x] ? r / group : 0;
+      const int64_t t = use.r.first + local[x];
+      const uint32_t place = ix.positions ? ix.positions[t] : use.r.cached + (uint32_t)local[x];
+      from[x] = ix.window > 0 && place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
+      if (live[x] && ix.window > 0 && place < use.r.cached) bad = true;
+      if (live[x]) from_most = max(from_most, from[x]);
+      m[x] = -INFINITY; l[x] = 0.0f; any[x] = false;
+      if (S::Q_IN_REGS) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(q.ptr + t * q.sn + (int64_t)(hk * group + (live[x] ? r % group : 0)) * q.sh);
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) { qf[k][x] = live[x] ? p[8 * k + pair] : 0u; qf[k][2 + x] = live[x] ? p[8 * k + 4 + pair] : 0u; }
+      }
+    }
+    if (ix.window > 0) from_most = __reduce_max_sync(0xffffffffu, from_most);
+    if (!S::Q_IN_REGS) {
+      __syncthreads();
+      for (int i = tid; i < TILE_ROWS * CHUNKS; i += TILE_WARPS * 32) {
+        const int r = i / CHUNKS, c = i % CHUNKS, g = row_tile * TILE_ROWS + r;
+        const bool has = g < use.r.fresh * group;
+        const T* p = q.ptr + (int64_t)(use.r.first + (has ? g / group : 0)) * q.sn + (int64_t)(hk * group + (has ? g % group : 0)) * q.sh + c * PER;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (has) v = *reinterpret_cast<const uint4*>(p);
+        *reinterpret_cast<uint4*>(q_tile + r * S::K_PITCH + c * PER) = v;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < OT; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
+  };
+  {
+    Place p[STAGES];                                                                                    // all look-ups, the queries, then the copies
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) if (i < todo) p[i] = look_up();
+    begin_unit(begin);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (i < todo) copy_block(i, p[i]);
+      copies_commit();
+    }
+    next_place = p[STAGES - 1];
+  }
 
   int stage = 0;
   for (int f = 0; f < todo; ++f) {
+    if (f > 0 && use.block == 0) begin_unit(begin + f);
     const int row_tile = use.row_tile, hk = use.hk;
-    if (f == 0 || use.block == 0) {                                                                     // a new unit: its rows
-      piece_begin = begin + f;
-      from_most = 0;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = row_tile * TILE_ROWS + 16 * mw + quad + 8 * x;
-        live[x] = r < use.r.fresh * group;
-        local[x] = live[x] ? r / group : 0;
-        const int64_t t = use.r.first + local[x];
-        const uint32_t place = ix.positions ? ix.positions[t] : use.r.cached + (uint32_t)local[x];
-        from[x] = ix.window > 0 && place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
-        if (live[x] && ix.window > 0 && place < use.r.cached) bad = true;
-        if (live[x]) from_most = max(from_most, from[x]);
-        m[x] = -INFINITY; l[x] = 0.0f; any[x] = false;
-        if (S::Q_IN_REGS) {
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(q.ptr + t * q.sn + (int64_t)(hk * group + (live[x] ? r % group : 0)) * q.sh);
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) { qf[k][x] = live[x] ? p[8 * k + pair] : 0u; qf[k][2 + x] = live[x] ? p[8 * k + 4 + pair] : 0u; }
-        }
-      }
-      if (ix.window > 0) from_most = __reduce_max_sync(0xffffffffu, from_most);
-      if (!S::Q_IN_REGS) {
-        __syncthreads();
-        for (int i = tid; i < TILE_ROWS * CHUNKS; i += TILE_WARPS * 32) {
-          const int r = i / CHUNKS, c = i % CHUNKS, g = row_tile * TILE_ROWS + r;
-          const bool has = g < use.r.fresh * group;
-          const T* p = q.ptr + (int64_t)(use.r.first + (has ? g / group : 0)) * q.sn + (int64_t)(hk * group + (has ? g % group : 0)) * q.sh + c * PER;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (has) v = *reinterpret_cast<const uint4*>(p);
-          *reinterpret_cast<uint4*>(q_tile + r * S::K_PITCH + c * PER) = v;
-        }
-        __syncthreads();
-      }
-#pragma unroll
-      for (int n = 0; n < OT; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
-    }
 
     copies_wait<STAGES - 2>();
     if (MW == 1) __syncwarp(); else __syncthreads();
     {                                                                                                   // the stage that the last block left
       const int next = f + STAGES - 1;
-      if (next < todo) { copy_block(stage == 0 ? STAGES - 1 : stage - 1); if (next + 1 < todo) look_up(); }
+      if (next < todo) { copy_block(stage == 0 ? STAGES - 1 : stage - 1, next_place); if (next + 1 < todo) next_place = look_up(); }
       copies_commit();
     }
     const T* kt = reinterpret_cast<const T*>(raw + stage * S::STAGE) + kw * KEYS * S::K_PITCH;
@@ -416,22 +465,25 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     bool poisoned = false;
     if (j0 + KEYS > use.r.cached || j0 < from_most) {
       sees = 0;
+#pragma unroll 1
+      for (int i = 0; i < 4 * NT; ++i) {                                                                // a loop, for the code's size: few blocks come here
+        const int x = (i >> 1) & 1;
+        const uint32_t j = j0 + 8 * (i >> 2) + 2 * pair + (i & 1), mine_from = x ? from[1] : from[0];
+        const uint32_t row = (uint32_t)(x ? local[1] : local[0]);
+        bool v = x ? live[1] : live[0];
+        if (j < use.r.cached) v = v && j >= mine_from;
+        else {
+          const uint32_t d = j - use.r.cached;
+          v = v && d < (uint32_t)use.r.fresh;
+          if (v) v = ix.masks ? (d >> 5) < (uint32_t)ix.words && (ix.masks[(int64_t)(use.r.first + row) * ix.words + (d >> 5)] >> (d & 31) & 1u) : d <= row;
+          if (v && ix.window > 0) v = (ix.positions ? ix.positions[use.r.first + d] : j) >= mine_from;
+        }
+        sees |= (uint32_t)v << i;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = e >> 1;
-          const uint32_t j = j0 + 8 * n + 2 * pair + (e & 1);
-          bool v = live[x];
-          if (j < use.r.cached) v = v && j >= from[x];
-          else {
-            const uint32_t d = j - use.r.cached;
-            v = v && d < (uint32_t)use.r.fresh;
-            if (v) v = ix.masks ? (d >> 5) < (uint32_t)ix.words && (ix.masks[(int64_t)(use.r.first + local[x]) * ix.words + (d >> 5)] >> (d & 31) & 1u) : d <= (uint32_t)local[x];
-            if (v && ix.window > 0) v = (ix.positions ? ix.positions[use.r.first + d] : j) >= from[x];
-          }
-          if (v) sees |= 1u << (4 * n + e); else s[n][e] = -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) if (!(sees >> (4 * n + e) & 1u)) s[n][e] = -INFINITY;
       }
       // a value that only some rows see must not reach the others as 0 x NaN: such a block's second product goes without the tensor cores
       const uint32_t* w = reinterpret_cast<const uint32_t*>(vt);
@@ -471,26 +523,27 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
 
     // ---- O += P V
     if (poisoned) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
 #pragma unroll 1
-        for (int k = 0; k < 8; ++k) {
-          const int from = (lane & ~3) | (k >> 1);
-          float p[2];
-          bool v[2];
+      for (int k = 0; k < KEYS; ++k) {                                                                  // the key's weights lie in s[0]: the tile moves on every eight keys
+        const int from_lane = (lane & ~3) | ((k & 7) >> 1);
+        float p[2];
+        bool v[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            p[x] = __shfl_sync(0xffffffffu, (k & 1) ? s[n][2 * x + 1] : s[n][2 * x], from);
-            v[x] = __shfl_sync(0xffffffffu, sees >> (4 * n + 2 * x + (k & 1)) & 1u, from);
+        for (int x = 0; x < 2; ++x) {
+          p[x] = __shfl_sync(0xffffffffu, (k & 1) ? s[0][2 * x + 1] : s[0][2 * x], from_lane);
+          v[x] = __shfl_sync(0xffffffffu, sees >> (4 * (k >> 3) + 2 * x + (k & 1)) & 1u, from_lane);
+        }
+#pragma unroll
+        for (int i = 0; i < OT; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float val = ldf(vt, k * S::V_PITCH + 8 * i + 2 * pair + (e & 1));
+            if (v[e >> 1]) o[i][e] = fmaf(p[e >> 1], val, o[i][e]);
           }
+        }
+        if ((k & 7) == 7) {
 #pragma unroll
-          for (int i = 0; i < OT; ++i) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float val = ldf(vt, (8 * n + k) * S::V_PITCH + 8 * i + 2 * pair + (e & 1));
-              if (v[e >> 1]) o[i][e] = fmaf(p[e >> 1], val, o[i][e]);
-            }
-          }
+          for (int n = 0; n + 1 < NT; ++n) { s[n][0] = s[n + 1][0]; s[n][1] = s[n + 1][1]; s[n][2] = s[n + 1][2]; s[n][3] = s[n + 1][3]; }
         }
       }
     } else if (!F32) {
@@ -536,40 +589,58 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         if (seen && m[x] == -INFINITY) l[x] = NAN;                                                      // every score -inf: what the formula gives
       }
       if (KW > 1) {                                                                                     // the warps that share a row tile add up in order
+        const int rows = min(16, use.r.fresh * group - row_tile * TILE_ROWS);                            // of a row tile of 16 (MW 1)
+        const bool at_once = MW == 1 && rows * (KW - 1) <= 16;                                           // all warps' rows fit next to one another
         float* jm = joint + 16 * D;
-        for (int w = 1; w < KW; ++w) {
-          for (int g = 0; g < MW; ++g) {
-            __syncthreads();
-            if (kw == w && mw == g) {
+        auto give = [&](int at) {
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int r = quad + 8 * x;
-                if (pair == 0) { jm[2 * r] = m[x]; jm[2 * r + 1] = l[x]; }
+          for (int x = 0; x < 2; ++x) {
+            const int r = quad + 8 * x;
+            if (!live[x]) continue;
+            if (pair == 0) { jm[2 * (at + r)] = m[x]; jm[2 * (at + r) + 1] = l[x]; }
 #pragma unroll
-                for (int n = 0; n < OT; ++n) *reinterpret_cast<float2*>(joint + r * D + 8 * n + 2 * pair) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
-              }
+            for (int n = 0; n < OT; ++n) *reinterpret_cast<float2*>(joint + (at + r) * D + 8 * n + 2 * pair) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+          }
+        };
+        auto take = [&](int at) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = at + quad + 8 * x;
+            if (!live[x]) continue;
+            const float m2 = jm[2 * r], l2 = jm[2 * r + 1], top = fmaxf(m[x], m2), base = top == -INFINITY ? 0.0f : top * c2;
+            const float ca = exp2_fast(fmaf(m[x], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
+            l[x] = l[x] * ca + l2 * cb;
+            m[x] = top;
+#pragma unroll
+            for (int n = 0; n < OT; ++n) {
+              const float2 v = *reinterpret_cast<const float2*>(joint + r * D + 8 * n + 2 * pair);
+              o[n][2 * x] = o[n][2 * x] * ca + v.x * cb;
+              o[n][2 * x + 1] = o[n][2 * x + 1] * ca + v.y * cb;
             }
-            __syncthreads();
-            if (kw == 0 && mw == g) {
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int r = quad + 8 * x;
-                const float m2 = jm[2 * r], l2 = jm[2 * r + 1], top = fmaxf(m[x], m2), base = top == -INFINITY ? 0.0f : top * c2;
-                const float ca = exp2_fast(fmaf(m[x], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
-                l[x] = l[x] * ca + l2 * cb;
-                m[x] = top;
-#pragma unroll
-                for (int n = 0; n < OT; ++n) {
-                  const float2 v = *reinterpret_cast<const float2*>(joint + r * D + 8 * n + 2 * pair);
-                  o[n][2 * x] = o[n][2 * x] * ca + v.x * cb;
-                  o[n][2 * x + 1] = o[n][2 * x + 1] * ca + v.y * cb;
-                }
-              }
+          }
+        };
+        __syncthreads();                                                                                 // what a unit before left has been taken
+        if (at_once) {
+          if (kw > 0) give((kw - 1) * rows);
+          __syncthreads();
+          if (kw == 0) {
+#pragma unroll 1
+            for (int w = 1; w < KW; ++w) take((w - 1) * rows);
+          }
+        } else {
+#pragma unroll 1
+          for (int w = 1; w < KW; ++w) {
+#pragma unroll 1
+            for (int g = 0; g < MW; ++g) {
+              if (kw == w && mw == g) give(0);
+              __syncthreads();
+              if (kw == 0 && mw == g) take(0);
+              __syncthreads();
             }
           }
         }
       }
-      const unsigned long long unit_begin = begin + f - use.block;
+      const uint32_t unit_begin = begin + f - use.block;
       const bool whole = unit_done && piece_begin == unit_begin;
       if (kw == 0) {
         const int slot = 2 * blockIdx.x + (piece_begin == unit_begin ? 1 : 0);
@@ -600,67 +671,112 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         }
       }
       if (!unit_done && piece_begin == unit_begin && tid == 0) {                                        // this CTA holds the unit's first piece
-        const unsigned long long unit_end = unit_begin + use.r.blocks, last = (unit_end * ctas + total - 1) / total - 1;
-        work.split[blockIdx.x] = SplitUnit{(int)(last - blockIdx.x) + 1, use.b, hk, row_tile};
+        work.split[blockIdx.x] = SplitUnit{(int)(share_of(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.b, hk, row_tile};
       }
     }
     use.step(ix, group, TILE_ROWS, kv_heads, &bad);
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (bad) raise_fault(fault, OP_PAGED_RANGE);
   else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
 }
 
-// Joins the pieces of the units that several CTAs shared: block (c, row) takes row `row` of the unit whose first piece CTA c left. Four warps walk the
-// pieces (a fixed order), lanes the columns.
+// Joins the pieces of the units that several CTAs shared: block c takes the unit whose first piece CTA c left. Its warps share out the rows, and where
+// there are fewer rows than warps the pieces of a row too (in a fixed order); lanes are columns. A warp's loads of eight pieces are in flight together.
+constexpr int JOIN_THREADS = 1024;
+
 template <class T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(JOIN_THREADS)
 paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, float scale, uint32_t* fault) {
-  __shared__ float acc[4][256], s_l[4], s_m[4];
+  constexpr int WARPS = JOIN_THREADS / 32;
+  __shared__ float s_l[WARPS], s_m[WARPS];
+  extern __shared__ float acc[];                                          // [WARPS][dim]
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const SplitUnit u = work.split[blockIdx.x];
   if (u.pieces == 0) return;
   const uint32_t first = ix.starts[u.request];
-  const int r = u.row_tile * tile_rows + blockIdx.y;
-  if (r >= (int)(ix.starts[u.request + 1] - first) * group) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rows = min(tile_rows, (int)(ix.starts[u.request + 1] - first) * group - u.row_tile * tile_rows);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int shares = 1;                                                         // warps to a row
+  while (2 * shares * rows <= WARPS && 2 * shares <= u.pieces) shares *= 2;
+  const int part = warp % shares, step = WARPS / shares;
   const float c2 = scale * 1.4426950408889634f;
-  auto row_of = [&](int p) { return (int64_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * tile_rows + blockIdx.y; };
-  float top = -INFINITY;
-  for (int p = tid; p < u.pieces; p += 128) top = fmaxf(top, work.ml[row_of(p)].x);
-  top = warp_max(top);
-  if (lane == 0) s_m[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const float base = top == -INFINITY ? 0.0f : top * c2;
-  float l = 0.0f, o[MAXI];
-#pragma unroll
-  for (int i = 0; i < MAXI; ++i) o[i] = 0.0f;
-#pragma unroll 4
-  for (int p = warp; p < u.pieces; p += 4) {
-    const int64_t row = row_of(p);
-    const float2 ml = work.ml[row];
-    const float w = exp2_fast(fmaf(ml.x, c2, -base));
-    l = fmaf(ml.y, w, l);
-#pragma unroll
-    for (int i = 0; i < MAXI; ++i) { const int d = lane + 32 * i; if (d < dim) o[i] = fmaf(work.o[row * dim + d], w, o[i]); }
-  }
-#pragma unroll
-  for (int i = 0; i < MAXI; ++i) { const int d = lane + 32 * i; if (d < dim) acc[warp][d] = o[i]; }
-  if (lane == 0) s_l[warp] = l;
-  __syncthreads();
-  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  const bool seen = !(top == -INFINITY && l == 0.0f);
-  const float inv = seen ? 1.0f / l : 0.0f;
-  const int64_t t = first + r / group;
-  const int h = u.kv_head * group + r % group;
-  T* po = out.ptr + t * out.sn + h * out.sh;
   bool wrong = false;
-  for (int d = tid; d < dim; d += 128) {
-    const float v = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
-    wrong |= !isfinite(v);
-    stf(po, d, v);
+  for (int r0 = 0; r0 < rows; r0 += step) {
+    const int r = r0 + warp / shares;
+    const bool live = r < rows;
+    auto row_of = [&](int p) { return (int64_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * tile_rows + r; };
+    float top = -INFINITY, l = 0.0f;
+    float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};     // columns 4 lane .. 4 lane + 3, and 128 more for a head of 256
+    if (live) {
+      for (int p = part + shares * lane; p < u.pieces; p += shares * 32) top = fmaxf(top, work.ml[row_of(p)].x);
+      top = warp_max(top);
+      const float base = top == -INFINITY ? 0.0f : top * c2;
+      for (int p0 = part; p0 < u.pieces; p0 += 8 * shares) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = 4 * lane + 128 * i;
+          if (128 * i >= dim) break;
+          float4 v[8];
+          float2 ml[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool there = p0 + k * shares < u.pieces;
+            v[k] = there && d < dim ? *reinterpret_cast<const float4*>(work.o + row_of(p0 + k * shares) * dim + d) : make_float4(0, 0, 0, 0);
+            ml[k] = there ? work.ml[row_of(p0 + k * shares)] : make_float2(-INFINITY, 0.0f);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float w = p0 + k * shares < u.pieces ? exp2_fast(fmaf(ml[k].x, c2, -base)) : 0.0f;
+            if (i == 0) l = fmaf(ml[k].y, w, l);
+            o[i].x = fmaf(v[k].x, w, o[i].x); o[i].y = fmaf(v[k].y, w, o[i].y); o[i].z = fmaf(v[k].z, w, o[i].z); o[i].w = fmaf(v[k].w, w, o[i].w);
+          }
+        }
+      }
+    }
+    if (shares > 1) {                                                     // the same for all warps: a block-wide exchange
+      if (lane == 0) { s_m[warp] = top; s_l[warp] = l; }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { const int d = 4 * lane + 128 * i; if (d < dim) *reinterpret_cast<float4*>(acc + warp * dim + d) = o[i]; }
+      __syncthreads();
+      if (part == 0 && live) {
+        for (int w = 1; w < shares; ++w) top = fmaxf(top, s_m[warp + w]);
+        const float base = top == -INFINITY ? 0.0f : top * c2;
+        l = 0.0f;
+        o[0] = o[1] = make_float4(0, 0, 0, 0);
+        for (int w = 0; w < shares; ++w) {
+          const float c = exp2_fast(fmaf(s_m[warp + w], c2, -base));
+          l = fmaf(s_l[warp + w], c, l);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int d = 4 * lane + 128 * i;
+            if (d >= dim) continue;
+            const float4 v = *reinterpret_cast<const float4*>(acc + (warp + w) * dim + d);
+            o[i].x = fmaf(v.x, c, o[i].x); o[i].y = fmaf(v.y, c, o[i].y); o[i].z = fmaf(v.z, c, o[i].z); o[i].w = fmaf(v.w, c, o[i].w);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (live && part == 0) {
+      const int g = u.row_tile * tile_rows + r;
+      const int64_t t = first + g / group;
+      const int h = u.kv_head * group + g % group;
+      const bool seen = !(top == -INFINITY && l == 0.0f);
+      const float inv = seen ? 1.0f / l : 0.0f;
+      T* po = out.ptr + t * out.sn + h * out.sh;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = 4 * lane + 128 * i;
+        if (d >= dim) continue;
+        const float4 v = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
+        wrong |= !isfinite(v.x) || !isfinite(v.y) || !isfinite(v.z) || !isfinite(v.w);
+        if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4*>(po + d) = v;
+        else *reinterpret_cast<uint2*>(po + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      }
+      if (lane == 0 && lse) lse[t * heads + h] = seen ? top * scale + logf(l) : -INFINITY;
+    }
   }
-  if (tid == 0 && lse) lse[t * heads + h] = seen ? top * scale + logf(l) : -INFINITY;
   if (wrong) raise_fault(fault, OP_PAGED_ATTN);
 }
 
@@ -685,10 +801,11 @@ ojc_status attn_dims(const char* op, const ojc_tensor* q, const ojc_tensor* k_pa
   return OJC_OK;
 }
 
-constexpr int MAX_CTAS = 2 * REDUCE_SMS;   // of the tiles kernel: the partition, and so the bits, do not depend on the opened device
+constexpr int MAX_CTAS = FINER * 2 * REDUCE_SMS;   // of the tiles kernel: the partition, and so the bits, do not depend on the opened device
 
 // The tiles kernel's workspace: the split units, then (m, l) and outputs of two row tiles (of 64 rows at most) for each CTA.
-uint64_t tiles_workspace(int64_t dim) { return 8192 + (uint64_t)2 * MAX_CTAS * 64 * (dim + 2) * 4; }
+constexpr uint64_t SPLIT_BYTES = (MAX_CTAS * sizeof(SplitUnit) + 255) / 256 * 256;
+uint64_t tiles_workspace(int64_t dim) { return SPLIT_BYTES + (uint64_t)2 * MAX_CTAS * 64 * (dim + 2) * 4; }
 
 // 16-byte rows: base and strides aligned
 bool rows_aligned(const ojc_tensor* t, int axes) {
@@ -717,18 +834,31 @@ ojc_status tiles_launch(const AttnCall& c) {
     OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tiles_kernel<T, D, MW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), c.op);
     attr[c.be->device] = true;
   }
-  const int ctas = TileShape<T, D, MW>::CTAS_PER_SM * REDUCE_SMS, group = (int)(c.a.heads / c.a.kv_heads);
+  const int wave = TileShape<T, D, MW>::CTAS_PER_SM * REDUCE_SMS, group = (int)(c.a.heads / c.a.kv_heads);
+  // no more CTAs than the longest requests that the tables allow would need: the grid never limits the number of shares
+  const int64_t tiles = (c.a.tokens * group + 16 * MW - 1) / (16 * MW) + c.ix.batch;
+  const unsigned long long most = (unsigned long long)tiles * (unsigned long long)c.a.kv_heads * (unsigned long long)(c.ix.width * c.ix.page / BLOCK_KEYS + 1);
+  const unsigned ctas = std::max(1u, tile_shares(most, (uint32_t)wave));
   TileWork w;
   w.split = (SplitUnit*)c.work;
-  w.ml = (float2*)((char*)c.work + 8192);
+  w.ml = (float2*)((char*)c.work + SPLIT_BYTES);
   w.o = (float*)(w.ml + (size_t)2 * MAX_CTAS * 64);
-  paged_attention_tiles_kernel<T, D, MW><<<ctas, TILE_WARPS * 32, smem, c.be->stream>>>(rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
-                                                                                       rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, (int)c.a.kv_heads, c.scale, c.be->fault_dev);
-  OJC_LAUNCHED(c.be, c.op);
+  // Both kernels are queued while the one before them still runs and wait for its end before they look at memory.
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, 16 * MW);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(TILE_WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = c.be->stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tiles_kernel<T, D, MW>, rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
+                                    rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, (int)c.a.kv_heads, wave, c.scale, c.be->fault_dev), c.op);
+  c.be->launches++;
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.dynamicSmemBytes = JOIN_THREADS / 32 * D * 4;
   OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T>, c.ix, rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, 16 * MW, D, c.scale, c.be->fault_dev), c.op);
   OJC_LAUNCHED(c.be, c.op);
   return OJC_OK;
