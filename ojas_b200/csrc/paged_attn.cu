@@ -6,20 +6,9 @@
 #include <type_traits>
 
 #include "dispatch.cuh"
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace {
-
-constexpr int MAXI = 8;  // head_dim <= 256: each lane owns columns lane + 32 i
-
-struct PassIndex {       // the pass's index tables (all U32)
-  const uint32_t *tables, *cached, *starts, *masks, *positions;
-  int batch, words;
-  int64_t tokens, width, pages;
-  uint32_t page;
-  int page_shift;        // log2 of the page, or -1
-  int64_t window;        // 0: none
-};
 
 // the last request that starts at or before token t (requests without tokens share their start with the next one)
 __device__ __forceinline__ int request_of(const uint32_t* starts, int batch, uint32_t t) {
@@ -53,10 +42,10 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
   const T* qp = q.ptr + t * q.sn + h * q.sh;
   for (int d = lane; d < dim; d += 32) qs[d] = ldf(qp, d);
   __syncwarp();
-  float m = -INFINITY, l = 0.0f, o[MAXI];
+  float m = -INFINITY, l = 0.0f, o[MAX_HEAD_COLUMNS];
   bool any = false;
 #pragma unroll
-  for (int i = 0; i < MAXI; ++i) o[i] = 0.0f;
+  for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) o[i] = 0.0f;
   for (int64_t j0 = min(low < 0 ? 0 : low + 1, cached); j0 < total; j0 += 32) {
     const int64_t j = j0 + lane;
     bool sees = j < total;
@@ -93,13 +82,13 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
     const float p = sees ? expf(s - m_new) : 0.0f;
     l = l * corr + warp_sum(p);
 #pragma unroll
-    for (int i = 0; i < MAXI; ++i) o[i] *= corr;
+    for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) o[i] *= corr;
     for (uint32_t left = seen; left; left &= left - 1) {
       const int jj = __ffs(left) - 1;
       const float pj = __shfl_sync(0xffffffffu, p, jj);
       const T* pv = vp.ptr + __shfl_sync(0xffffffffu, at, jj) + hk * vp.sh;
 #pragma unroll
-      for (int i = 0; i < MAXI; ++i) { const int d = lane + 32 * i; if (d < dim) o[i] = fmaf(pj, ldf(pv, d), o[i]); }
+      for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) { const int d = lane + 32 * i; if (d < dim) o[i] = fmaf(pj, ldf(pv, d), o[i]); }
     }
     m = m_new;
   }
@@ -107,7 +96,7 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
   const float inv = any ? 1.0f / l : 0.0f;
   T* po = out.ptr + t * out.sn + h * out.sh;
 #pragma unroll
-  for (int i = 0; i < MAXI; ++i) {
+  for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) {
     const int d = lane + 32 * i;
     if (d < dim) { const float v = any ? o[i] * inv : 0.0f; wrong |= !isfinite(v); stf(po, d, v); }
   }
@@ -117,19 +106,12 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 }
 
 // ======================================================================== tiles on the tensor cores
-// A unit of work is (request, KV head, row tile): the rows of a KV head are its request's tokens times the query heads of the group (token-major), cut
-// into tiles of 16 * MW; its keys are walked in blocks of 64. All units' blocks in a row are one line of work that the CTAs share out evenly, whatever
-// the lengths: a CTA that gets the middle of a unit leaves (maximum, sum, unnormalised output) per row in the workspace, and a second small kernel joins
-// the pieces of a unit in order. Every CTA finds its own stretch from the lengths, so nothing is planned on the host and nothing read back.
+// Row tiles of 16 * MW rows, key blocks of 64 (paged_attn.cuh has the line of work).
 //
 // What bounds it: the cache's bytes for few rows. Four warps to a CTA, two CTAs to an SM, three stages of 64 keys each, rows fetched by 16-byte asynchronous
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
 // Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
-#ifndef SHARE_FINER
-#define SHARE_FINER 1
-#define SHARE_LONG 24
-#endif
 constexpr int BLOCK_KEYS = 64, TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -150,8 +132,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 // x = hi + lo up to 2^-22 |x|, both TF32
 __device__ __forceinline__ void split_tf32(float x, uint32_t* hi, uint32_t* lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*hi) : "f"(x));
@@ -159,41 +139,6 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t* hi, uint32_t* lo) 
 }
 __device__ __forceinline__ float quad_max(float v) { v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1)); return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)); }
 __device__ __forceinline__ float quad_sum(float v) { v += __shfl_xor_sync(0xffffffffu, v, 1); return v + __shfl_xor_sync(0xffffffffu, v, 2); }
-
-// What a unit that several CTAs share leaves for the joining kernel: its pieces are slot 2c + 1 of its first CTA c and slots 2(c + 1), 2(c + 2), ...
-struct SplitUnit { int pieces, request, kv_head, row_tile; };
-struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][16 MW][D], ml [2 CTAs][16 MW], split [CTAs]
-
-struct Request { uint32_t cached, first; int fresh, first_block, blocks, row_tiles; };
-__device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int group, int tile_rows, bool* bad) {
-  Request r;
-  const uint32_t first = ix.starts[b], end = ix.starts[b + 1], cached = ix.cached[b];
-  const bool wrong = end < first || end > ix.tokens || (int64_t)cached + (int64_t)(end - first) > ix.width * ix.page;
-  *bad |= wrong;
-  r.cached = wrong ? 0 : cached;
-  r.first = first;
-  r.fresh = wrong ? 0 : (int)(end - first);
-  const int64_t from = ix.window > 0 ? (int64_t)r.cached - ix.window + 1 : 0;   // positions of new tokens are at least `cached`
-  r.first_block = from > 0 ? (int)(from / BLOCK_KEYS) : 0;
-  r.blocks = r.fresh == 0 ? 0 : (int)((r.cached + (uint32_t)r.fresh + BLOCK_KEYS - 1) / BLOCK_KEYS) - r.first_block;
-  r.row_tiles = (int)((uint32_t)(r.fresh * group + tile_rows - 1) / (uint32_t)tile_rows);
-  return r;
-}
-
-// A place on the line of work; all threads of a CTA hold the same one.
-struct Cursor {
-  Request r;
-  int b, hk, row_tile, block;     // block counts from 0
-  __device__ __forceinline__ void step(const PassIndex& ix, int group, int tile_rows, int kv_heads, bool* bad) {
-    if (++block < r.blocks) return;
-    block = 0;
-    if (++row_tile < r.row_tiles) return;
-    row_tile = 0;
-    if (++hk < kv_heads) return;
-    hk = 0;
-    do { if (++b >= ix.batch) return; r = load_request(ix, b, group, tile_rows, bad); } while (r.blocks == 0);
-  }
-};
 
 template <class T, int D, int MW> struct TileShape {
   static constexpr int K_PITCH = std::is_same<T, float>::value ? D + 4 : D + 8, V_PITCH = D + 8;   // elements: odd multiples of 16 bytes (ldmatrix), or 4 and 8 banks a row (F32 fragments)
@@ -205,19 +150,10 @@ template <class T, int D, int MW> struct TileShape {
   static constexpr int CTAS_PER_SM = SMEM <= 112 * 1024 + 512 ? 2 : 1;
 };
 
-// Shares of the line of work: at least two blocks each up to one wave of CTAs (`wave`: what the GPU holds at once); beyond that up to FINER waves of
-// shares of at least LONG_SHARE blocks, since SMs do not stream equally fast and the later waves go to those that are done.
-constexpr uint32_t FINER = SHARE_FINER, LONG_SHARE = SHARE_LONG;
-__host__ __device__ __forceinline__ uint32_t tile_shares(unsigned long long blocks, uint32_t wave) {
-  const unsigned long long few = (blocks + 1) / 2, many = blocks / LONG_SHARE;
-  const unsigned long long n = few < wave ? few : many < wave ? wave : many;
-  return (uint32_t)(n < (unsigned long long)FINER * wave ? n : (unsigned long long)FINER * wave);
-}
-
 template <class T, int D, int MW>
 __global__ void __launch_bounds__(TILE_WARPS * 32, TileShape<T, D, MW>::CTAS_PER_SM)
 paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesView<const T> vp, PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads,
-                             int group, int kv_heads, int wave, float scale, uint32_t* fault) {
+                             int group, int kv_heads, float scale, uint32_t* fault) {
   using S = TileShape<T, D, MW>;
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr int STAGES = S::STAGES;
@@ -228,79 +164,19 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   float* joint = reinterpret_cast<float*>(raw + STAGES * S::STAGE);                                   // [16][D] and [16] (m, l): the warps' outputs meet here
   uint64_t* rows_at = reinterpret_cast<uint64_t*>(raw + STAGES * S::STAGE + S::JOINT);
   T* q_tile = reinterpret_cast<T*>(rows_at + TILE_WARPS * 32);                                          // only without Q_IN_REGS
-  __shared__ uint32_t s_sum[TILE_WARPS], s_at;
-  __shared__ int s_b;
-  __shared__ Request s_r;
+  __shared__ ShareScratch s_share;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
   bool bad = false, wrong = false;
-
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // ---- this CTA's stretch [begin, end) of the line of work: the blocks in all, an equal share of them, and the request in which the share begins
-  auto blocks_of = [&](const Request& r) {
-    const unsigned long long n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
-    bad |= n >= 1ull << 31;
-    return n >= 1ull << 31 ? 0u : (uint32_t)n;
-  };
-  auto scan = [&](uint32_t n, uint32_t* before) {                                                        // of a chunk of 128 requests; the sum comes back
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const uint32_t a = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += a; }
-    __syncthreads();
-    if (lane == 31) s_sum[warp] = n;
-    __syncthreads();
-    *before = n;
-    uint32_t sum = 0;
-#pragma unroll
-    for (int w = 0; w < TILE_WARPS; ++w) { if (w < warp) *before += s_sum[w]; sum += s_sum[w]; }
-    return sum;
-  };
-  Request mine_r = {};
-  uint32_t mine_n = 0, mine_at = 0, total = 0;
-  for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {
-    mine_r = {};
-    mine_n = 0;
-    if (b0 + tid < ix.batch) { mine_r = load_request(ix, b0 + tid, group, TILE_ROWS, &bad); mine_n = blocks_of(mine_r); }
-    const uint32_t sum = scan(mine_n, &mine_at);
-    bad |= total + sum < total || total + sum >= 1u << 31;
-    total = bad && (total + sum < total || total + sum >= 1u << 31) ? total : total + sum;
-  }
-  const uint32_t ctas = min(gridDim.x, tile_shares(total, wave));
   if (tid == 0) work.split[blockIdx.x] = SplitUnit{0, 0, 0, 0};
+  Share<BLOCK_KEYS> share;
+  const bool any_work = find_share<BLOCK_KEYS, TILE_WARPS * 32>(ix, group, TILE_ROWS, kv_heads, &s_share, &share, &bad);
   if (bad) raise_fault(fault, OP_PAGED_RANGE);
-  if (blockIdx.x >= ctas) return;
-  const uint32_t share = total / ctas, longer = total - share * ctas;                                    // the first `longer` shares have one block more
-  auto share_begin = [&](uint32_t c) { return c * share + min(c, longer); };
-  auto share_of = [&](uint32_t block) { return block < longer * (share + 1) ? block / (share + 1) : longer + (block - longer * (share + 1)) / share; };
-  const uint32_t begin = share_begin(blockIdx.x), end = share_begin(blockIdx.x + 1);
-  if (ix.batch <= TILE_WARPS * 32) {
-    mine_at -= mine_n;
-    if (mine_n && mine_at <= begin && begin - mine_at < mine_n) { s_b = tid; s_at = mine_at; s_r = mine_r; }
-    __syncthreads();
-  } else {
-    uint32_t carry = 0;
-    for (int b0 = 0; b0 < ix.batch; b0 += TILE_WARPS * 32) {
-      uint32_t n = 0, at;
-      Request r = {};
-      if (b0 + tid < ix.batch) { r = load_request(ix, b0 + tid, group, TILE_ROWS, &bad); n = blocks_of(r); }
-      const uint32_t sum = scan(n, &at);
-      at += carry - n;
-      if (n && at <= begin && begin - at < n) { s_b = b0 + tid; s_at = at; s_r = r; }
-      __syncthreads();
-      carry += sum;
-      if (carry > begin) break;
-    }
-  }
-  Cursor use;
-  use.b = s_b;
-  use.r = s_r;
-  {
-    const uint32_t unit = (begin - s_at) / (uint32_t)use.r.blocks;
-    use.block = (int)(begin - s_at - unit * (uint32_t)use.r.blocks);
-    use.hk = (int)(unit / (uint32_t)use.r.row_tiles);
-    use.row_tile = (int)(unit - (uint32_t)use.hk * (uint32_t)use.r.row_tiles);
-  }
-  Cursor ahead = use;                                                                                   // the block whose pages are looked up next
-  const int todo = (int)(end - begin);
+  if (!any_work) return;
+  const uint32_t begin = share.begin;
+  const int todo = share.todo;
+  Cursor<BLOCK_KEYS> use = share.at;
+  Cursor<BLOCK_KEYS> ahead = use;                                                                                   // the block whose pages are looked up next
 
   // ---- copies: warp w fetches keys 16 w .. 16 w + 15 of a block; lane l looks up key l's row of K, lane 16 + l its row of V. Places behind the last
   // one repeat it: what lies there is masked like any place that is not seen.
@@ -352,7 +228,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   uint32_t from[2], from_most = 0;                                                                      // the first position in a row's window
   int local[2];
   bool live[2];
-  const float c2 = scale * 1.4426950408889634f;
+  const float c2 = scale * LOG2_E;
   uint32_t piece_begin = begin;
   Place next_place;
   auto begin_unit = [&](uint32_t at) {                                                                   // a new unit: its rows
@@ -664,14 +540,14 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
             if (pair == 0 && lse) lse[t * heads + h] = seen ? m[x] * scale + logf(l[x]) : -INFINITY;
           } else {
             const int64_t row = (int64_t)slot * TILE_ROWS + 16 * mw + quad + 8 * x;
-            if (pair == 0) work.ml[row] = make_float2(m[x], l[x]);
+            if (pair == 0) work.ml[row] = make_float2(m[x] * c2, l[x]);
 #pragma unroll
             for (int n = 0; n < OT; ++n) *reinterpret_cast<float2*>(work.o + row * D + 8 * n + 2 * pair) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
           }
         }
       }
       if (!unit_done && piece_begin == unit_begin && tid == 0) {                                        // this CTA holds the unit's first piece
-        work.split[blockIdx.x] = SplitUnit{(int)(share_of(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.b, hk, row_tile};
+        work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.b, hk, row_tile};
       }
     }
     use.step(ix, group, TILE_ROWS, kv_heads, &bad);
@@ -687,7 +563,7 @@ constexpr int JOIN_THREADS = 1024;
 
 template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS)
-paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, float scale, uint32_t* fault) {
+paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, uint32_t* fault) {
   constexpr int WARPS = JOIN_THREADS / 32;
   __shared__ float s_l[WARPS], s_m[WARPS];
   extern __shared__ float acc[];                                          // [WARPS][dim]
@@ -700,7 +576,6 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
   int shares = 1;                                                         // warps to a row
   while (2 * shares * rows <= WARPS && 2 * shares <= u.pieces) shares *= 2;
   const int part = warp % shares, step = WARPS / shares;
-  const float c2 = scale * 1.4426950408889634f;
   bool wrong = false;
   for (int r0 = 0; r0 < rows; r0 += step) {
     const int r = r0 + warp / shares;
@@ -711,7 +586,7 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
     if (live) {
       for (int p = part + shares * lane; p < u.pieces; p += shares * 32) top = fmaxf(top, work.ml[row_of(p)].x);
       top = warp_max(top);
-      const float base = top == -INFINITY ? 0.0f : top * c2;
+      const float base = top == -INFINITY ? 0.0f : top;
       for (int p0 = part; p0 < u.pieces; p0 += 8 * shares) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -727,7 +602,7 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
           }
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float w = p0 + k * shares < u.pieces ? exp2_fast(fmaf(ml[k].x, c2, -base)) : 0.0f;
+            const float w = p0 + k * shares < u.pieces ? exp2_fast(ml[k].x - base) : 0.0f;
             if (i == 0) l = fmaf(ml[k].y, w, l);
             o[i].x = fmaf(v[k].x, w, o[i].x); o[i].y = fmaf(v[k].y, w, o[i].y); o[i].z = fmaf(v[k].z, w, o[i].z); o[i].w = fmaf(v[k].w, w, o[i].w);
           }
@@ -741,11 +616,11 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
       __syncthreads();
       if (part == 0 && live) {
         for (int w = 1; w < shares; ++w) top = fmaxf(top, s_m[warp + w]);
-        const float base = top == -INFINITY ? 0.0f : top * c2;
+        const float base = top == -INFINITY ? 0.0f : top;
         l = 0.0f;
         o[0] = o[1] = make_float4(0, 0, 0, 0);
         for (int w = 0; w < shares; ++w) {
-          const float c = exp2_fast(fmaf(s_m[warp + w], c2, -base));
+          const float c = exp2_fast(s_m[warp + w] - base);
           l = fmaf(s_l[warp + w], c, l);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -774,7 +649,7 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
         if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4*>(po + d) = v;
         else *reinterpret_cast<uint2*>(po + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
       }
-      if (lane == 0 && lse) lse[t * heads + h] = seen ? top * scale + logf(l) : -INFINITY;
+      if (lane == 0 && lse) lse[t * heads + h] = seen ? top * LN_2 + logf(l) : -INFINITY;
     }
   }
   if (wrong) raise_fault(fault, OP_PAGED_ATTN);
@@ -787,25 +662,21 @@ ojc_status u32_table(const char* op, const char* what, const ojc_tensor* t, int 
   return OJC_OK;
 }
 
-struct AttnDims { int64_t tokens, heads, kv_heads, dim, pages, page; };
-
 ojc_status attn_dims(const char* op, const ojc_tensor* q, const ojc_tensor* k_pages, AttnDims* a) {
   OJC_TRY(check_tensor(op, "q", q, false)); OJC_TRY(check_tensor(op, "k_pages", k_pages, false));
   if (q->rank != 3 || k_pages->rank != 4 || q->shape[2] != k_pages->shape[3]) return ojc_fail(OJC_ERR_SHAPE, op, "q [N, H, D]; k_pages, v_pages [P, page, Hkv, D]");
   *a = AttnDims{q->shape[0], q->shape[1], k_pages->shape[2], q->shape[2], k_pages->shape[0], k_pages->shape[1]};
   if (numel(q) == 0 || numel(k_pages) == 0) return ojc_fail(OJC_ERR_SHAPE, op, "empty tensor");
   if (a->heads % a->kv_heads != 0) return ojc_fail(OJC_ERR_SHAPE, op, "heads must be a multiple of KV heads");
-  if (a->dim > 32 * MAXI) return ojc_fail(OJC_ERR_UNSUPPORTED_HEAD_DIM, op, "head_dim above 256");
+  if (a->dim > 32 * MAX_HEAD_COLUMNS) return ojc_fail(OJC_ERR_UNSUPPORTED_HEAD_DIM, op, "head_dim above 256");
   if (a->tokens > INT32_MAX / a->heads || a->page > (1 << 24) || a->pages > (int64_t)OJC_NONE / a->page) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "extent out of range");
   if (q->dtype != k_pages->dtype || !is_float(q)) return ojc_fail(OJC_ERR_DTYPE, op, "q and the pages share F32 or BF16");
   return OJC_OK;
 }
 
-constexpr int MAX_CTAS = FINER * 2 * REDUCE_SMS;   // of the tiles kernel: the partition, and so the bits, do not depend on the opened device
-
-// The tiles kernel's workspace: the split units, then (m, l) and outputs of two row tiles (of 64 rows at most) for each CTA.
-constexpr uint64_t SPLIT_BYTES = (MAX_CTAS * sizeof(SplitUnit) + 255) / 256 * 256;
-uint64_t tiles_workspace(int64_t dim) { return SPLIT_BYTES + (uint64_t)2 * MAX_CTAS * 64 * (dim + 2) * 4; }
+// The workspace: the split units, then (m, l) and outputs of two row tiles for each CTA.
+constexpr uint64_t SPLIT_BYTES = (MAX_SHARES * sizeof(SplitUnit) + 255) / 256 * 256;
+uint64_t attn_workspace(int64_t dim) { return SPLIT_BYTES + (uint64_t)2 * MAX_SHARE_ROWS * (dim + 2) * 4; }
 
 // 16-byte rows: base and strides aligned
 bool rows_aligned(const ojc_tensor* t, int axes) {
@@ -820,48 +691,32 @@ bool tiles_take(const ojc_tensor* q, const ojc_tensor* k, const ojc_tensor* v, c
   return shape && rows_aligned(q, 2) && rows_aligned(k, 3) && rows_aligned(v, 3) && rows_aligned(out, 2);
 }
 
-struct AttnCall {
-  ojc_backend* be; const char* op;
-  const ojc_tensor *q, *k, *v; ojc_tensor* out; float* lse;
-  PassIndex ix; AttnDims a; float scale; void* work;
-};
-
 template <class T, int D, int MW>
 ojc_status tiles_launch(const AttnCall& c) {
-  constexpr int smem = TileShape<T, D, MW>::SMEM;
+  using S = TileShape<T, D, MW>;
   static PerDeviceFlag attr;
   if (!attr[c.be->device]) {
-    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tiles_kernel<T, D, MW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), c.op);
+    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tiles_kernel<T, D, MW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), c.op);
     attr[c.be->device] = true;
   }
-  const int wave = TileShape<T, D, MW>::CTAS_PER_SM * REDUCE_SMS, group = (int)(c.a.heads / c.a.kv_heads);
-  // no more CTAs than the longest requests that the tables allow would need: the grid never limits the number of shares
-  const int64_t tiles = (c.a.tokens * group + 16 * MW - 1) / (16 * MW) + c.ix.batch;
-  const unsigned long long most = (unsigned long long)tiles * (unsigned long long)c.a.kv_heads * (unsigned long long)(c.ix.width * c.ix.page / BLOCK_KEYS + 1);
-  const unsigned ctas = std::max(1u, tile_shares(most, (uint32_t)wave));
-  TileWork w;
-  w.split = (SplitUnit*)c.work;
-  w.ml = (float2*)((char*)c.work + SPLIT_BYTES);
-  w.o = (float*)(w.ml + (size_t)2 * MAX_CTAS * 64);
-  // Both kernels are queued while the one before them still runs and wait for its end before they look at memory.
+  static_assert(S::CTAS_PER_SM * REDUCE_SMS <= MAX_SHARES && S::CTAS_PER_SM * REDUCE_SMS * 16 * MW <= MAX_SHARE_ROWS, "workspace");
+  const unsigned ctas = S::CTAS_PER_SM * REDUCE_SMS;
+  const int group = (int)(c.a.heads / c.a.kv_heads);
+  // queued while the kernel before still runs; it waits for that one's end before it looks at memory
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(TILE_WARPS * 32);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = c.be->stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
   OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tiles_kernel<T, D, MW>, rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
-                                    rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, (int)c.a.kv_heads, wave, c.scale, c.be->fault_dev), c.op);
+                                    rows_view<T>(c.out), c.lse, c.work, (int)c.a.heads, group, (int)c.a.kv_heads, c.scale, c.be->fault_dev), c.op);
   c.be->launches++;
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.dynamicSmemBytes = JOIN_THREADS / 32 * D * 4;
-  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T>, c.ix, rows_view<T>(c.out), c.lse, w, (int)c.a.heads, group, 16 * MW, D, c.scale, c.be->fault_dev), c.op);
-  OJC_LAUNCHED(c.be, c.op);
-  return OJC_OK;
+  return paged_attention_join(c, ctas, 16 * MW);
 }
 
 template <class T, int D>
@@ -886,6 +741,26 @@ ojc_status tiles_by_dim(const AttnCall& c) {
 
 }  // namespace
 
+ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(shares);
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.dynamicSmemBytes = JOIN_THREADS / 32 * c.a.dim * 4;
+  cfg.stream = c.be->stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const int group = (int)(c.a.heads / c.a.kv_heads), heads = (int)c.a.heads, dim = (int)c.a.dim;
+  if (c.q->dtype == OJC_F32)
+    OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<float>, c.ix, rows_view<float>(c.out), c.lse, c.work, heads, group, tile_rows, dim, c.be->fault_dev), c.op);
+  else
+    OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<bf16>, c.ix, rows_view<bf16>(c.out), c.lse, c.work, heads, group, tile_rows, dim, c.be->fault_dev), c.op);
+  OJC_LAUNCHED(c.be, c.op);
+  return OJC_OK;
+}
+
 extern "C" {
 
 ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, uint64_t* bytes) {
@@ -894,7 +769,7 @@ ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor
   if (!bytes) return ojc_fail(OJC_ERR_BACKEND, op, "null out pointer");
   AttnDims a;
   OJC_TRY(attn_dims(op, q, k_pages, &a));
-  *bytes = tiles_workspace(a.dim);
+  *bytes = attn_workspace(a.dim);
   return OJC_OK;
 }
 
@@ -942,7 +817,11 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
                      (a.page & (a.page - 1)) ? -1 : __builtin_ctzll((unsigned long long)a.page), window < 0 ? 0 : window};
   const float scale = 1.0f / sqrtf((float)a.dim);
   float* lse_out = lse ? (float*)lse->data : nullptr;
-  const AttnCall call{be, op, q, k_pages, v_pages, out, lse_out, ix, a, scale, workspace};
+  TileWork work;
+  work.split = (SplitUnit*)workspace;
+  work.ml = (float2*)((char*)workspace + SPLIT_BYTES);
+  work.o = (float*)(work.ml + (size_t)2 * MAX_SHARE_ROWS);
+  const AttnCall call{be, op, q, k_pages, v_pages, out, lse_out, ix, a, scale, work};
   const bool tiles = tiles_take(q, k_pages, v_pages, out, a.dim);
   return dispatch_float(op, q->dtype, [&](auto t) {
     using T = decltype(t);

@@ -1,0 +1,155 @@
+// Shared by the attention kernels over a paged KV cache: the pass's index tables, the line of work that CTAs share out, and what they leave for the join.
+//
+// A unit of work is (request, KV head, row tile): the rows of a KV head are its request's tokens times the query heads of the group (token-major), cut
+// into tiles; its keys are walked in blocks. All units' blocks in a row are one line of work that the CTAs share out evenly, whatever the lengths: a CTA
+// that gets the middle of a unit leaves (maximum, sum, unnormalised output) per row in the workspace, and a second small kernel joins the pieces of a
+// unit in order. Every CTA finds its own stretch from the lengths, so nothing is planned on the host and nothing read back; the shares depend on lengths
+// and shapes alone, and so do the bits.
+#pragma once
+#include "paged.cuh"
+
+constexpr int MAX_HEAD_COLUMNS = 8;  // head_dim <= 256: each lane owns columns lane + 32 i
+
+struct PassIndex {       // the pass's index tables (all U32)
+  const uint32_t *tables, *cached, *starts, *masks, *positions;
+  int batch, words;
+  int64_t tokens, width, pages;
+  uint32_t page;
+  int page_shift;        // log2 of the page, or -1
+  int64_t window;        // 0: none
+};
+
+// What a unit that several CTAs share leaves for the joining kernel: its pieces are slot 2c + 1 of its first CTA c and slots 2(c + 1), 2(c + 2), ...
+struct SplitUnit { int pieces, request, kv_head, row_tile; };
+struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][tile rows][D]; ml [2 CTAs][tile rows]: maximum in log2 units, sum; split [CTAs]
+
+// Both kernels' limits: one wave of CTAs (two to an SM of the tiles kernel with 64 rows at most, one of the tcgen05 kernel with 256)
+constexpr int MAX_SHARES = 2 * REDUCE_SMS, MAX_SHARE_ROWS = REDUCE_SMS * 256;
+
+struct AttnDims { int64_t tokens, heads, kv_heads, dim, pages, page; };
+struct AttnCall {
+  ojc_backend* be; const char* op;
+  const ojc_tensor *q, *k, *v; ojc_tensor* out; float* lse;
+  PassIndex ix; AttnDims a; float scale; TileWork work;
+};
+// The joining kernel behind one that ran `shares` CTAs with tiles of `tile_rows` rows
+ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows);
+// tcgen05 / TMEM form (BF16, head_dim 64 or 128, pages that tile 128 keys): `taken` says whether it was launched
+bool paged_attention_tcgen05_takes(const AttnCall& c);
+ojc_status paged_attention_tcgen05(const AttnCall& c, int tiles);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+constexpr float LOG2_E = 1.4426950408889634f, LN_2 = 0.6931471805599453f;
+
+struct Request { uint32_t cached, first; int fresh, first_block, blocks, row_tiles; };
+template <int KEYS>
+__device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int group, int tile_rows, bool* bad) {
+  Request r;
+  const uint32_t first = ix.starts[b], end = ix.starts[b + 1], cached = ix.cached[b];
+  const bool wrong = end < first || end > ix.tokens || (int64_t)cached + (int64_t)(end - first) > ix.width * ix.page;
+  *bad |= wrong;
+  r.cached = wrong ? 0 : cached;
+  r.first = first;
+  r.fresh = wrong ? 0 : (int)(end - first);
+  const int64_t from = ix.window > 0 ? (int64_t)r.cached - ix.window + 1 : 0;   // positions of new tokens are at least `cached`
+  r.first_block = from > 0 ? (int)(from / KEYS) : 0;
+  r.blocks = r.fresh == 0 ? 0 : (int)((r.cached + (uint32_t)r.fresh + KEYS - 1) / KEYS) - r.first_block;
+  r.row_tiles = (int)((uint32_t)(r.fresh * group + tile_rows - 1) / (uint32_t)tile_rows);
+  return r;
+}
+
+// A place on the line of work; all threads of a CTA hold the same one.
+template <int KEYS>
+struct Cursor {
+  Request r;
+  int b, hk, row_tile, block;     // block counts from 0
+  __device__ __forceinline__ void step(const PassIndex& ix, int group, int tile_rows, int kv_heads, bool* bad) {
+    if (++block < r.blocks) return;
+    block = 0;
+    if (++row_tile < r.row_tiles) return;
+    row_tile = 0;
+    if (++hk < kv_heads) return;
+    hk = 0;
+    do { if (++b >= ix.batch) return; r = load_request<KEYS>(ix, b, group, tile_rows, bad); } while (r.blocks == 0);
+  }
+};
+
+// One CTA's stretch of the line: `todo` blocks from number `begin` on, the first of them at `at`. The first `longer` of the `ctas` shares have
+// `share` + 1 blocks, the others `share`.
+template <int KEYS>
+struct Share {
+  uint32_t begin, ctas, share, longer;
+  int todo;
+  Cursor<KEYS> at;
+  __device__ __forceinline__ uint32_t begin_of(uint32_t c) const { return c * share + min(c, longer); }
+  __device__ __forceinline__ uint32_t of_block(uint32_t block) const { return block < longer * (share + 1) ? block / (share + 1) : longer + (block - longer * (share + 1)) / share; }
+};
+struct ShareScratch { uint32_t sum[32], at; int b; Request r; };
+
+// Called by all THREADS threads of the CTA; false: nothing for it to do. Lengths are read once for up to THREADS requests, twice beyond.
+template <int KEYS, int THREADS>
+__device__ __forceinline__ bool find_share(const PassIndex& ix, int group, int tile_rows, int kv_heads, ShareScratch* sh, Share<KEYS>* out, bool* bad) {
+  constexpr int WARPS = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto blocks_of = [&](const Request& r) {
+    const unsigned long long n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
+    *bad |= n >= 1ull << 31;
+    return n >= 1ull << 31 ? 0u : (uint32_t)n;
+  };
+  auto scan = [&](uint32_t n, uint32_t* upto) {                  // of a chunk of requests; the chunk's sum comes back
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const uint32_t a = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += a; }
+    __syncthreads();
+    if (lane == 31) sh->sum[warp] = n;
+    __syncthreads();
+    *upto = n;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) { if (w < warp) *upto += sh->sum[w]; sum += sh->sum[w]; }
+    return sum;
+  };
+  Request mine = {};
+  uint32_t n = 0, upto = 0, total = 0;
+  for (int b0 = 0; b0 < ix.batch; b0 += THREADS) {
+    mine = {};
+    n = 0;
+    if (b0 + tid < ix.batch) { mine = load_request<KEYS>(ix, b0 + tid, group, tile_rows, bad); n = blocks_of(mine); }
+    const uint32_t sum = scan(n, &upto);
+    if ((unsigned long long)total + sum < 1ull << 31) total += sum; else *bad = true;
+  }
+  out->ctas = min(gridDim.x, (total + 1) / 2);                   // at least two blocks each
+  if (blockIdx.x >= out->ctas) return false;
+  out->share = total / out->ctas;
+  out->longer = total - out->share * out->ctas;
+  const uint32_t begin = out->begin = out->begin_of(blockIdx.x);
+  out->todo = (int)(out->begin_of(blockIdx.x + 1) - begin);
+  if (ix.batch <= THREADS) {
+    upto -= n;
+    if (n && upto <= begin && begin - upto < n) { sh->b = tid; sh->at = upto; sh->r = mine; }
+    __syncthreads();
+  } else {
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < ix.batch; b0 += THREADS) {
+      mine = {};
+      n = 0;
+      if (b0 + tid < ix.batch) { mine = load_request<KEYS>(ix, b0 + tid, group, tile_rows, bad); n = blocks_of(mine); }
+      const uint32_t sum = scan(n, &upto);
+      upto += carry - n;
+      if (n && upto <= begin && begin - upto < n) { sh->b = b0 + tid; sh->at = upto; sh->r = mine; }
+      __syncthreads();
+      carry += sum;
+      if (carry > begin) break;
+    }
+  }
+  Cursor<KEYS>& c = out->at;
+  c.b = sh->b;
+  c.r = sh->r;
+  const uint32_t unit = (begin - sh->at) / (uint32_t)c.r.blocks;
+  c.block = (int)(begin - sh->at - unit * (uint32_t)c.r.blocks);
+  c.hk = (int)(unit / (uint32_t)c.r.row_tiles);
+  c.row_tile = (int)(unit - (uint32_t)c.hk * (uint32_t)c.r.row_tiles);
+  return true;
+}
+#endif
