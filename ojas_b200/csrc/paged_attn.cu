@@ -719,10 +719,14 @@ ojc_status tiles_launch(const AttnCall& c) {
   return paged_attention_join(c, ctas, 16 * MW);
 }
 
+#ifndef ROWS_TC
+#define ROWS_TC 32
+#endif
 template <class T, int D>
 ojc_status tiles_by_rows(const AttnCall& c) {
   // rows of a KV head in a request of average length: what the host knows without a readback
   const int64_t rows = (c.a.tokens + c.ix.batch - 1) / c.ix.batch * (c.a.heads / c.a.kv_heads);
+  if ((D == 64 || D == 128) && rows > ROWS_TC && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
   if (rows <= 16) return tiles_launch<T, D, 1>(c);
   if (rows <= 32) return tiles_launch<T, D, 2>(c);
   return tiles_launch<T, D, 4>(c);

@@ -34,7 +34,7 @@ struct AttnCall {
 };
 // The joining kernel behind one that ran `shares` CTAs with tiles of `tile_rows` rows
 ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows);
-// tcgen05 / TMEM form (BF16, head_dim 64 or 128, pages that tile 128 keys): `taken` says whether it was launched
+// tcgen05 / TMEM form with one or two tiles of 128 rows (BF16, head_dim 64 or 128, pages that tile 128 keys)
 bool paged_attention_tcgen05_takes(const AttnCall& c);
 ojc_status paged_attention_tcgen05(const AttnCall& c, int tiles);
 

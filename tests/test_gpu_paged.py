@@ -345,6 +345,13 @@ def test_attention_in_a_window(be, cached, new, h, hk, d, page, window, bf16, tr
     Case(window, cached, new, h, hk, d, page, tree, bf16).check(be, window=window)
 
 
+@pytest.mark.parametrize("cached,new,h,hk,d,page", [([4000, 2100], [63, 40], 16, 16, 128, 32), ([3000, 4100], [33, 127], 16, 16, 64, 64), ([2500, 1, 900], [100, 3, 130], 8, 4, 128, 16),
+                                                    ([5000], [45], 24, 24, 128, 128), ([3900], [20], 12, 12, 64, 16), ([6000], [12], 8, 8, 96, 16)])
+def test_attention_with_many_key_blocks_to_a_share(be, cached, new, h, hk, d, page):
+    """Several units and key blocks to each CTA of every kernel: the rings and barriers go round more than once, warps without rows run beside others."""
+    Case(21, cached, new, h, hk, d, page, True, True).check(be)
+
+
 @pytest.mark.parametrize("bf16", [True, False])
 @pytest.mark.parametrize("h,hk,d", [(8, 2, 128), (4, 4, 64), (3, 1, 40)])
 def test_attention_layouts_and_workspaces_give_the_same_bits(be, bf16, h, hk, d):
