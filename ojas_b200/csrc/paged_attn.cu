@@ -168,7 +168,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
   bool bad = false, wrong = false;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid == 0) work.split[blockIdx.x] = SplitUnit{0, 0, 0, 0};
+  if (tid == 0) work.split[blockIdx.x].pieces = 0;
   Share<BLOCK_KEYS> share;
   const bool any_work = find_share<BLOCK_KEYS, TILE_WARPS * 32>(ix, group, TILE_ROWS, kv_heads, &s_share, &share, &bad);
   if (bad) raise_fault(fault, OP_PAGED_RANGE);
@@ -547,7 +547,8 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         }
       }
       if (!unit_done && piece_begin == unit_begin && tid == 0) {                                        // this CTA holds the unit's first piece
-        work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.b, hk, row_tile};
+        work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, hk, row_tile * TILE_ROWS,
+                                               min(TILE_ROWS, use.r.fresh * group - row_tile * TILE_ROWS), use.r.first};
       }
     }
     use.step(ix, group, TILE_ROWS, kv_heads, &bad);
@@ -557,73 +558,82 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
 }
 
-// Joins the pieces of the units that several CTAs shared: block c takes the unit whose first piece CTA c left. Its warps share out the rows, and where
-// there are fewer rows than warps the pieces of a row too (in a fixed order); lanes are columns. A warp's loads of eight pieces are in flight together.
-constexpr int JOIN_THREADS = 1024;
+// Joins the pieces of the units that several CTAs shared: blocks (c, .) take the unit whose first piece CTA c left. A warp takes a row, or where a unit has
+// many pieces a 2nd, 4th or 8th part of a row's (joined in a fixed order); lanes are columns. The loads of four pieces, maxima and outputs, are in
+// flight together: two round trips to memory for a unit of up to four pieces (latency is all there is to this kernel, so registers are kept few: with
+// eight pieces at 110 registers it took three times as long for units of 256 rows). COLS: 128 columns of four to a lane.
+constexpr int JOIN_WARPS = 8, JOIN_PIECES = 4;
 
-template <class T>
-__global__ void __launch_bounds__(JOIN_THREADS)
-paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, uint32_t* fault) {
-  constexpr int WARPS = JOIN_THREADS / 32;
-  __shared__ float s_l[WARPS], s_m[WARPS];
-  extern __shared__ float acc[];                                          // [WARPS][dim]
+template <class T, int COLS>
+__global__ void __launch_bounds__(JOIN_WARPS * 32, COLS == 1 ? 6 : 4)
+paged_attention_join_kernel(RowsView<T> out, float* __restrict__ lse, TileWork work, int heads, int group, int tile_rows, int dim, uint32_t* fault) {
+  __shared__ float s_l[JOIN_WARPS], s_m[JOIN_WARPS];
+  extern __shared__ float acc[];                                          // [JOIN_WARPS][dim]
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const SplitUnit u = work.split[blockIdx.x];
   if (u.pieces == 0) return;
-  const uint32_t first = ix.starts[u.request];
-  const int rows = min(tile_rows, (int)(ix.starts[u.request + 1] - first) * group - u.row_tile * tile_rows);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int shares = 1;                                                         // warps to a row
-  while (2 * shares * rows <= WARPS && 2 * shares <= u.pieces) shares *= 2;
-  const int part = warp % shares, step = WARPS / shares;
+  while (shares < JOIN_WARPS && shares * JOIN_PIECES < u.pieces) shares *= 2;
+  const int part = warp % shares, step = JOIN_WARPS / shares;
   bool wrong = false;
-  for (int r0 = 0; r0 < rows; r0 += step) {
+  for (int r0 = blockIdx.y * step; r0 < u.rows; r0 += gridDim.y * step) {
     const int r = r0 + warp / shares;
-    const bool live = r < rows;
-    auto row_of = [&](int p) { return (int64_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * tile_rows + r; };
-    float top = -INFINITY, l = 0.0f;
-    float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};     // columns 4 lane .. 4 lane + 3, and 128 more for a head of 256
-    if (live) {
-      for (int p = part + shares * lane; p < u.pieces; p += shares * 32) top = fmaxf(top, work.ml[row_of(p)].x);
-      top = warp_max(top);
-      const float base = top == -INFINITY ? 0.0f : top;
-      for (int p0 = part; p0 < u.pieces; p0 += 8 * shares) {
+    const bool live = r < u.rows;
+    float top = -INFINITY, l = 0.0f;                                      // maxima in log2 units
+    float4 o[COLS];                                                       // columns 4 lane .. 4 lane + 3, and 128 more for a head of 256
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < COLS; ++i) o[i] = make_float4(0, 0, 0, 0);
+    for (int p0 = part; live && p0 < u.pieces; p0 += JOIN_PIECES * shares) {
+      float4 v[COLS][JOIN_PIECES];
+      float2 ml[JOIN_PIECES];
+#pragma unroll
+      for (int k = 0; k < JOIN_PIECES; ++k) {
+        const int p = p0 + k * shares;
+        const bool there = p < u.pieces;
+        const int64_t row = (int64_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * tile_rows + r;
+        ml[k] = there ? work.ml[row] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) {
           const int d = 4 * lane + 128 * i;
-          if (128 * i >= dim) break;
-          float4 v[8];
-          float2 ml[8];
+          v[i][k] = there && d < dim ? *reinterpret_cast<const float4*>(work.o + row * dim + d) : make_float4(0, 0, 0, 0);
+        }
+      }
+      float most = top;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const bool there = p0 + k * shares < u.pieces;
-            v[k] = there && d < dim ? *reinterpret_cast<const float4*>(work.o + row_of(p0 + k * shares) * dim + d) : make_float4(0, 0, 0, 0);
-            ml[k] = there ? work.ml[row_of(p0 + k * shares)] : make_float2(-INFINITY, 0.0f);
-          }
+      for (int k = 0; k < JOIN_PIECES; ++k) most = fmaxf(most, ml[k].x);
+      const float base = most == -INFINITY ? 0.0f : most, c = exp2_fast(top - base);
+      l *= c;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float w = p0 + k * shares < u.pieces ? exp2_fast(ml[k].x - base) : 0.0f;
-            if (i == 0) l = fmaf(ml[k].y, w, l);
-            o[i].x = fmaf(v[k].x, w, o[i].x); o[i].y = fmaf(v[k].y, w, o[i].y); o[i].z = fmaf(v[k].z, w, o[i].z); o[i].w = fmaf(v[k].w, w, o[i].w);
-          }
+      for (int i = 0; i < COLS; ++i) { o[i].x *= c; o[i].y *= c; o[i].z *= c; o[i].w *= c; }
+      top = most;
+#pragma unroll
+      for (int k = 0; k < JOIN_PIECES; ++k) {
+        if (p0 + k * shares >= u.pieces) break;
+        const float w = exp2_fast(ml[k].x - base);
+        l = fmaf(ml[k].y, w, l);
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) {
+          o[i].x = fmaf(v[i][k].x, w, o[i].x); o[i].y = fmaf(v[i][k].y, w, o[i].y); o[i].z = fmaf(v[i][k].z, w, o[i].z); o[i].w = fmaf(v[i][k].w, w, o[i].w);
         }
       }
     }
     if (shares > 1) {                                                     // the same for all warps: a block-wide exchange
       if (lane == 0) { s_m[warp] = top; s_l[warp] = l; }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) { const int d = 4 * lane + 128 * i; if (d < dim) *reinterpret_cast<float4*>(acc + warp * dim + d) = o[i]; }
+      for (int i = 0; i < COLS; ++i) { const int d = 4 * lane + 128 * i; if (d < dim) *reinterpret_cast<float4*>(acc + warp * dim + d) = o[i]; }
       __syncthreads();
       if (part == 0 && live) {
         for (int w = 1; w < shares; ++w) top = fmaxf(top, s_m[warp + w]);
         const float base = top == -INFINITY ? 0.0f : top;
         l = 0.0f;
-        o[0] = o[1] = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) o[i] = make_float4(0, 0, 0, 0);
         for (int w = 0; w < shares; ++w) {
           const float c = exp2_fast(s_m[warp + w] - base);
           l = fmaf(s_l[warp + w], c, l);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < COLS; ++i) {
             const int d = 4 * lane + 128 * i;
             if (d >= dim) continue;
             const float4 v = *reinterpret_cast<const float4*>(acc + (warp + w) * dim + d);
@@ -634,14 +644,14 @@ paged_attention_join_kernel(PassIndex ix, RowsView<T> out, float* __restrict__ l
       __syncthreads();
     }
     if (live && part == 0) {
-      const int g = u.row_tile * tile_rows + r;
-      const int64_t t = first + g / group;
+      const int g = u.row + r;
+      const int64_t t = u.first + g / group;
       const int h = u.kv_head * group + g % group;
       const bool seen = !(top == -INFINITY && l == 0.0f);
       const float inv = seen ? 1.0f / l : 0.0f;
       T* po = out.ptr + t * out.sn + h * out.sh;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < COLS; ++i) {
         const int d = 4 * lane + 128 * i;
         if (d >= dim) continue;
         const float4 v = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
@@ -750,17 +760,19 @@ ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_row
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(shares);
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.dynamicSmemBytes = JOIN_THREADS / 32 * c.a.dim * 4;
+  cfg.gridDim = dim3(shares, tile_rows / (tile_rows <= 64 ? 4 : 8));   // rows go round: any grid does, these leave a warp one row of most units
+  cfg.blockDim = dim3(JOIN_WARPS * 32);
+  cfg.dynamicSmemBytes = JOIN_WARPS * c.a.dim * 4;
   cfg.stream = c.be->stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
   const int group = (int)(c.a.heads / c.a.kv_heads), heads = (int)c.a.heads, dim = (int)c.a.dim;
-  if (c.q->dtype == OJC_F32)
-    OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<float>, c.ix, rows_view<float>(c.out), c.lse, c.work, heads, group, tile_rows, dim, c.be->fault_dev), c.op);
-  else
-    OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<bf16>, c.ix, rows_view<bf16>(c.out), c.lse, c.work, heads, group, tile_rows, dim, c.be->fault_dev), c.op);
+  auto run = [&](auto t, auto kernel) {
+    using T = decltype(t);
+    return cudaLaunchKernelEx(&cfg, kernel, rows_view<T>(c.out), c.lse, c.work, heads, group, tile_rows, dim, c.be->fault_dev);
+  };
+  OJC_CUDA(c.be, c.q->dtype == OJC_F32 ? run(float(), paged_attention_join_kernel<float, 1>) : dim <= 128 ? run(bf16(), paged_attention_join_kernel<bf16, 1>)
+                                       : run(bf16(), paged_attention_join_kernel<bf16, 2>), c.op);   // the F32 tiles end at 128 columns
   OJC_LAUNCHED(c.be, c.op);
   return OJC_OK;
 }

@@ -20,7 +20,8 @@ struct PassIndex {       // the pass's index tables (all U32)
 };
 
 // What a unit that several CTAs share leaves for the joining kernel: its pieces are slot 2c + 1 of its first CTA c and slots 2(c + 1), 2(c + 2), ...
-struct SplitUnit { int pieces, request, kv_head, row_tile; };
+// `first` is the token of the request's row 0, `row` the tile's first row, `rows` how many it has.
+struct SplitUnit { int pieces, kv_head, row, rows; uint32_t first; };
 struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][tile rows][D]; ml [2 CTAs][tile rows]: maximum in log2 units, sum; split [CTAs]
 
 // Both kernels' limits: one wave of CTAs (two to an SM of the tiles kernel with 64 rows at most, one of the tcgen05 kernel with 256)

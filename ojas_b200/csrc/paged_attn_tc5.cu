@@ -129,7 +129,7 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid == 0) args.work.split[blockIdx.x] = SplitUnit{0, 0, 0, 0};
+  if (tid == 0) args.work.split[blockIdx.x].pieces = 0;
   bool bad = false;
   Share<KEYS> share;
   const bool any_work = find_share<KEYS, C::THREADS>(ix, args.group, TILE_ROWS, args.kv_heads, &s_share, &share, &bad);
@@ -462,7 +462,8 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
           if (row.live && !whole) args.work.ml[at] = make_float2(have ? m : -INFINITY, l);
         }
         if (!unit_done && starts && tid == 0)
-          args.work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.b, use.hk, use.row_tile};
+          args.work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.hk, use.row_tile * TILE_ROWS,
+                                                    min(TILE_ROWS, use.r.fresh * args.group - use.row_tile * TILE_ROWS), use.r.first};
       }
       use.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
     }
