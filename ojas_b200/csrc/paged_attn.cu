@@ -730,7 +730,7 @@ ojc_status tiles_launch(const AttnCall& c) {
 }
 
 #ifndef ROWS_TC
-#define ROWS_TC 32
+#define ROWS_TC 16
 #endif
 template <class T, int D>
 ojc_status tiles_by_rows(const AttnCall& c) {

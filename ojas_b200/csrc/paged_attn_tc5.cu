@@ -61,42 +61,61 @@ struct TcArgs {
   TileWork work;
   int heads, group, kv_heads;
   int k_heads_inside, v_heads_inside;   // tensor-map order: (D, Hkv, page, P) or (D, page, Hkv, P)
+  int out_sectors;                      // out's rows start at 32-byte boundaries
   int box_rows;                         // rows of a page that one box holds: min(page, 128)
   float scale;
   uint32_t* fault;
 };
 
-// What a row sees of the 32 places from j on, as bits
+// What a row sees of the 128 places from j on, as bits: the row's mask words are loaded together, then shifted to the places
 struct RowMask { uint32_t local, from; bool live; };
-__device__ __forceinline__ uint32_t seen_bits(const PassIndex& ix, const Request& r, const RowMask& row, uint32_t j) {
-  if (!row.live) return 0;
-  uint32_t bits = 0;
-  if (j < r.cached) {
-    const uint32_t n = r.cached - j;
-    bits = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-    if (row.from > j) bits &= row.from - j >= 32 ? 0u : 0xffffffffu << (row.from - j);
-    if (n >= 32) return bits;
-  }
-  // new tokens: number d0 at bit `shift`
-  const uint32_t shift = j < r.cached ? r.cached - j : 0, d0 = j < r.cached ? 0 : j - r.cached;
-  uint32_t fresh;
+__device__ __forceinline__ void seen_bits(const PassIndex& ix, const Request& r, const RowMask& row, uint32_t j, uint32_t (&bits)[4]) {
+  const int32_t d0 = (int32_t)(j - r.cached);                  // the first place's number among the new tokens (below 0: cached)
+  uint32_t m[5] = {0, 0, 0, 0, 0};
   if (ix.masks) {
-    const uint32_t* m = ix.masks + (int64_t)(r.first + row.local) * ix.words;
-    const uint32_t w = d0 >> 5;
-    const uint32_t lo = w < (uint32_t)ix.words ? m[w] : 0u, hi = w + 1 < (uint32_t)ix.words ? m[w + 1] : 0u;
-    fresh = __funnelshift_r(lo, hi, d0 & 31);
-  } else {
-    fresh = row.local < d0 ? 0u : row.local - d0 >= 31 ? 0xffffffffu : (2u << (row.local - d0)) - 1u;
+    const uint32_t* p = ix.masks + (int64_t)(r.first + row.local) * ix.words;
+    const int32_t w0 = d0 >> 5;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) if (row.live && w0 + k >= 0 && w0 + k < ix.words) m[k] = p[w0 + k];
   }
-  const uint32_t there = (uint32_t)r.fresh > d0 ? (uint32_t)r.fresh - d0 : 0u;
-  if (there < 32) fresh &= (1u << there) - 1u;
-  if (ix.window > 0) {
-    for (uint32_t left = fresh; left; left &= left - 1) {
-      const uint32_t e = __ffs(left) - 1, d = d0 + e;
-      if ((ix.positions ? ix.positions[r.first + d] : r.cached + d) < row.from) fresh &= ~(1u << e);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int32_t d = d0 + 32 * k;                             // this word's first place
+    auto below = [&](int64_t n) { return n <= d ? 0u : n >= (int64_t)d + 32 ? 0xffffffffu : (1u << (uint32_t)(n - d)) - 1u; };   // places with numbers under n
+    uint32_t fresh = ix.masks ? __funnelshift_r(m[k], m[k + 1], d0 & 31) : below((int64_t)row.local + 1);
+    fresh &= below(r.fresh) & ~below(0);
+    uint32_t old = below(0);
+    if (ix.window > 0) {
+      old &= ~below((int64_t)row.from - r.cached);
+      for (uint32_t left = fresh; left; left &= left - 1) {
+        const uint32_t e = __ffs(left) - 1, n = (uint32_t)d + e;
+        if ((ix.positions ? ix.positions[r.first + n] : r.cached + n) < row.from) fresh &= ~(1u << e);
+      }
     }
+    bits[k] = row.live ? old | fresh : 0u;
   }
-  return bits | fresh << shift;
+}
+
+// A store of 32 bytes: a whole sector to a thread, where a warp's threads write to rows of their own
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// A warp's 32 rows of a Q tile, asynchronously into the swizzled operand at `tile` (row pointers from the lanes that own the rows). Not inlined: it runs once
+// to a unit, and its addresses would cost the softmax loop its registers.
+template <int D>
+__device__ __noinline__ void fetch_q_rows(RowsView<const bf16> q, uint32_t first, int fresh, int hk, int row0, int group, uint32_t tile) {
+  const int lane = threadIdx.x & 31, t0 = threadIdx.x & 96, n = row0 + t0 + lane;
+  const uint64_t mine = n < fresh * group ? (uint64_t)(q.ptr + (int64_t)(first + (uint32_t)(n / group)) * q.sn + (int64_t)(hk * group + n % group) * q.sh) : 0;
+  const int c = lane % (D / 8);
+  const uint32_t dst = tile + (c >> 3) * SUB_BYTES + t0 * 128;
+#pragma unroll 4
+  for (int i = 0; i < D / 8; ++i) {
+    const int row = i * (256 / D) + lane / (D / 8);
+    const uint64_t from = __shfl_sync(0xffffffffu, mine, row);
+    if (from) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(from + c * 16) : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 template <int D, int T>
@@ -109,6 +128,7 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
   const uint32_t base = smem_u32(smem_raw);
   __shared__ ShareScratch s_share;
   __shared__ uint32_t s_found[3], s_from[8];
+  __shared__ Share<KEYS> s_line;
   const PassIndex& ix = args.ix;
   uint32_t* const fault = args.fault;
   auto bar = [&](int i) { return base + C::OFF_BAR + 8u * i; };
@@ -131,14 +151,20 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tid == 0) args.work.split[blockIdx.x].pieces = 0;
   bool bad = false;
-  Share<KEYS> share;
-  const bool any_work = find_share<KEYS, C::THREADS>(ix, args.group, TILE_ROWS, args.kv_heads, &s_share, &share, &bad);
+  int todo = 0;
+  Cursor<KEYS> use;
+  {
+    Share<KEYS> share;
+    if (find_share<KEYS, C::THREADS>(ix, args.group, TILE_ROWS, args.kv_heads, &s_share, &share, &bad)) {
+      todo = share.todo;
+      use = share.at;
+      if (tid == 0) s_line = share;
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int todo = any_work ? share.todo : 0;
-  Cursor<KEYS> use = share.at;
 
   // T 2: launched with 168 registers a thread (384 x 168 = 64,512); two softmax warpgroups of 216 and one of 72 take 128 x (2 x 216 + 72) = 64,512
   if (warp >= 4 * T) {
@@ -198,13 +224,17 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
     if (lane == 0) {
       const uint32_t idesc_s = make_idesc(ROWS, KEYS, 0, 0), idesc_pv = make_idesc(ROWS, D, 0, 1);
       const uint32_t q_lo = desc_lo(base, 0), k_lo = desc_lo(base + C::OFF_K, 0), v_lo = desc_lo(base + C::OFF_V, SUB_BYTES);
+      // The roles' loops together have to stay small for the instruction cache (the softmax warps waited for instructions more than for anything else). With T 1,
+      // where the MMA thread has time, its products are rolled loops at one site each (trees of 63 67 -> 62 us); with T 2 it is on the way, and they are not
+      // (213 us against 231).
+      constexpr int UNROLL = T == 1 ? 2 : 8;
       int units = 0;                                             // units begun so far: their Q tiles' barrier phase
       auto issue_s = [&](int g, int f, bool first) -> bool {     // S of block f for tile g
         const uint32_t s = f % STAGES, col = T == 1 ? (f & 1) * 128 : g * 128;
         if (first && !mbar_wait(bar(C::QFULL + g), units & 1, fault, abort_flag)) return false;
         if (!mbar_wait(bar(C::KFULL + s), (f / STAGES) & 1, fault, abort_flag)) return false;
         fence_after();
-#pragma unroll
+#pragma unroll UNROLL
         for (uint32_t kk = 0; kk < D / 16; ++kk)
           umma_lh(tmem_base + col, q_lo + g * TILE16 + (kk >> 2) * SUB16 + (kk & 3) * KSTEP, k_lo + s * TILE16 + (kk >> 2) * SUB16 + (kk & 3) * KSTEP, HI, idesc_s, kk > 0);
         umma_commit(bar(C::SFULL + (T == 1 ? f & 1 : g)));
@@ -216,29 +246,40 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
         if (!mbar_wait(bar(C::PREADY + (T == 1 ? f & 1 : g)), T == 1 ? (f >> 1) & 1 : f & 1, fault, abort_flag)) return false;
         if (!mbar_wait(bar(C::VFULL + s), (f / STAGES) & 1, fault, abort_flag)) return false;
         fence_after();
-#pragma unroll
+#pragma unroll UNROLL
         for (uint32_t kk = 0; kk < KEYS / 16; ++kk) umma_a_tmem(tmem_base + C::COL_O + g * D, tmem_base + col + kk * 8, v_lo + s * TILE16 + kk * MNSTEP, HI, idesc_pv);
         umma_commit(bar(C::PVFULL + g));
         if (g == T - 1) umma_commit(bar(C::VEMPTY + s));
         return true;
       };
       bool ok = true;
-      for (int g = 0; g < T && ok && todo > 0; ++g) ok = issue_s(g, 0, true);
-      for (int f = 0; f < todo && ok; ++f) {
-        const bool unit_ends = use.block + 1 == use.r.blocks, more = f + 1 < todo;
-        use.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
-        if (unit_ends) {
-          // the next unit's Q comes from rows that first wait for this unit's last O: both tiles' products before either's S
-          for (int g = 0; g < T && ok; ++g) ok = issue_pv(g, f);
-          ++units;
-          for (int g = 0; g < T && ok && more; ++g) ok = issue_s(g, f + 1, true);
-        } else if (T == 1) {
-          if (more) ok = issue_s(0, f + 1, false);               // the other S buffer, under this block's softmax
-          if (ok) ok = issue_pv(0, f);
-        } else {
-          for (int g = 0; g < T && ok; ++g) {
-            ok = issue_pv(g, f);
-            if (ok && more) ok = issue_s(g, f + 1, false);       // over the P just consumed: the pipe runs the two in order
+      if constexpr (T == 1) {
+        for (int f = -1; f < todo && ok; ++f) {
+          const bool begins = f < 0 || use.block + 1 == use.r.blocks, more = f + 1 < todo;   // the next block begins a unit (or the first one)
+          if (f >= 0) use.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
+#pragma unroll 1
+          for (int k = 0; k < 2 && ok; ++k) {
+            // the next S goes first, into the other buffer, under this block's softmax; but before a unit's first S the last P V of the one before: its Q
+            // comes from rows that first wait for that
+            if ((k == 0) != begins) { if (more) ok = issue_s(0, f + 1, begins); }
+            else if (f >= 0) { ok = issue_pv(0, f); units += begins; }
+          }
+        }
+      } else {
+        for (int g = 0; g < T && ok && todo > 0; ++g) ok = issue_s(g, 0, true);
+        for (int f = 0; f < todo && ok; ++f) {
+          const bool unit_ends = use.block + 1 == use.r.blocks, more = f + 1 < todo;
+          use.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
+          if (unit_ends) {
+            // the next unit's Q comes from rows that first wait for this unit's last O: both tiles' products before either's S
+            for (int g = 0; g < T && ok; ++g) ok = issue_pv(g, f);
+            ++units;
+            for (int g = 0; g < T && ok && more; ++g) ok = issue_s(g, f + 1, true);
+          } else {
+            for (int g = 0; g < T && ok; ++g) {
+              ok = issue_pv(g, f);
+              if (ok && more) ok = issue_s(g, f + 1, false);       // over the P just consumed: the pipe runs the two in order
+            }
           }
         }
       }
@@ -253,28 +294,34 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
     float m = 0.0f, l = 0.0f;
     bool have = false, any = false, wrong = false, ok = true;
     RowMask row = {0, 0, false};
-    uint32_t from_most = 0, piece_begin = share.begin;
-    int votes = 0, syncs = 0, h = 0;
-    int64_t token = 0;
+    uint32_t from_most = 0;
+    int votes = 0, syncs = 0, piece = 0;                          // piece: the block at which this CTA's piece of the unit begins
     auto sync_rows = [&]() -> bool {                              // all softmax threads, bounded
       mbar_arrive(bar(C::SYNC));
       return mbar_wait(bar(C::SYNC), syncs++ & 1, fault, abort_flag);
     };
+    // The Q tile of a unit: a warp fetches its 32 rows together (row pointers from the lanes that own them), asynchronously, straight into the swizzled
+    // operand. It is called as soon as the last S of the unit before is there, so the copies run under that unit's last softmax.
+    auto fetch_q = [&](const Cursor<KEYS>& u) { fetch_q_rows<D>(args.q, u.r.first, u.r.fresh, u.hk, u.row_tile * TILE_ROWS + g * ROWS, args.group, base + g * C::TILE_BYTES); };
+    auto give_q = [&]() {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      fence_async_smem();
+      mbar_arrive(bar(C::QFULL + g));
+    };
+    if (todo > 0) { fetch_q(use); give_q(); }
     for (int f = 0; f < todo && ok; ++f) {
       const uint32_t stage = f % STAGES;
       if (f == 0 || use.block == 0) {
         // ---- a new unit: this thread's row
-        piece_begin = share.begin + f;
+        piece = f;
         const int n = use.row_tile * TILE_ROWS + g * ROWS + t;
         row.live = n < use.r.fresh * args.group;
         row.local = row.live ? (uint32_t)(n / args.group) : 0u;
-        token = use.r.first + row.local;
-        h = use.hk * args.group + (row.live ? n % args.group : 0);
         row.from = 0;
         m = l = 0.0f;
         have = any = false;
         if (ix.window > 0) {
-          const uint32_t place = ix.positions ? ix.positions[token] : use.r.cached + row.local;
+          const uint32_t place = ix.positions ? ix.positions[use.r.first + row.local] : use.r.cached + row.local;
           if (row.live && place < use.r.cached) bad = true;
           row.from = place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
           const uint32_t most = __reduce_max_sync(0xffffffffu, row.live ? row.from : 0u);
@@ -285,14 +332,6 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
 #pragma unroll
           for (int w = 0; w < 4 * T; ++w) from_most = max(from_most, s_from[w]);
         }
-        if (row.live) {
-          const uint4* p = reinterpret_cast<const uint4*>(args.q.ptr + token * args.q.sn + h * args.q.sh);
-          uint8_t* dst = smem_raw + g * C::TILE_BYTES + t * 128;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * SUB_BYTES + (((c & 7) ^ (t & 7)) << 4)) = p[c];
-        }
-        fence_async_smem();
-        mbar_arrive(bar(C::QFULL + g));
         uint32_t zero[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) zero[e] = 0;
@@ -304,8 +343,11 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
       const uint32_t s_addr = lane_base + (T == 1 ? (f & 1) * 128 : g * 128);
       const uint32_t j0 = (uint32_t)(use.r.first_block + use.block) * KEYS, places = use.r.cached + (uint32_t)use.r.fresh;
       const bool masked = j0 + KEYS > use.r.cached || j0 < from_most;
+      const bool unit_done = use.block + 1 == use.r.blocks;
       bool poisoned = false;
+      uint32_t bits[4];
       if (masked) {
+        seen_bits(ix, use.r, row, j0, bits);
         // V's rows behind the last place become zeros; the others are searched for values that are not finite
         if (!mbar_wait(bar(C::VFULL + stage), (f / STAGES) & 1, fault, abort_flag)) { ok = false; break; }
         uint32_t odd = 0;
@@ -333,6 +375,11 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
       }
       if (!mbar_wait(bar(C::SFULL + (T == 1 ? f & 1 : g)), T == 1 ? (f >> 1) & 1 : f & 1, fault, abort_flag)) { ok = false; break; }
       fence_after();
+      if (unit_done && f + 1 < todo) {                            // every S that reads this unit's Q is there
+        Cursor<KEYS> next = use;
+        next.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
+        fetch_q(next);
+      }
       if (warp_live) {
         uint32_t r[KEYS];
 #pragma unroll
@@ -341,10 +388,9 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
         if (masked) {
 #pragma unroll
           for (int w = 0; w < KEYS / 32; ++w) {
-            const uint32_t bits = seen_bits(ix, use.r, row, j0 + 32 * w);
-            any |= bits != 0;
+            any |= bits[w] != 0;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) if (!(bits >> e & 1u)) r[32 * w + e] = 0xff800000u;
+            for (int e = 0; e < 32; ++e) if (!(bits[w] >> e & 1u)) r[32 * w + e] = 0xff800000u;
           }
         } else any = true;
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -360,10 +406,10 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
           have |= grow;
           m = m_new;
           l *= corr;
-          if (f > 0 && use.block != 0 && piece_begin != share.begin + f) {
+          if (f != piece) {
             if (!mbar_wait(bar(C::PVFULL + g), (f - 1) & 1, fault, abort_flag)) { ok = false; break; }   // O of the blocks before has landed
             fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(o_addr + c * 32, o);
@@ -391,12 +437,11 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
       }
       if (poisoned) {
         // ---- every row adds its own share of what is not finite, then the operand's are replaced by zeros
-        const bool before = f > 0 && piece_begin != share.begin + f;
-        if (before) { if (!mbar_wait(bar(C::PVFULL + g), (f - 1) & 1, fault, abort_flag)) { ok = false; break; } fence_after(); }
+        if (f != piece) { if (!mbar_wait(bar(C::PVFULL + g), (f - 1) & 1, fault, abort_flag)) { ok = false; break; } fence_after(); }
         const uint8_t* v = smem_raw + C::OFF_V + stage * C::TILE_BYTES;
 #pragma unroll 1
         for (int k = 0; k < KEYS && warp_live; ++k) {
-          const bool sees = seen_bits(ix, use.r, row, j0 + (k & ~31)) >> (k & 31) & 1u;
+          const bool sees = (k < 64 ? k < 32 ? bits[0] : bits[1] : k < 96 ? bits[2] : bits[3]) >> (k & 31) & 1u;
           const uint32_t pw = tmem_ld1(s_addr + (k >> 1));
           tmem_wait_ld();
           const float p = __uint_as_float((k & 1) ? pw & 0xffff0000u : pw << 16);
@@ -420,49 +465,58 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
         fence_async_smem();
         if (!sync_rows()) { ok = false; break; }
       }
+      // A parity tells two phases apart only for one who knows that the phase before has passed and the one behind it has not: with T 1 this block's S may
+      // be there before the last block's P V, so whoever is about to wait for this block's P V waits for the last one's first, while P is still held back.
+      if (T == 1 && f > 0 && (unit_done || f + 1 == todo) && !mbar_wait(bar(C::PVFULL + g), (f - 1) & 1, fault, abort_flag)) { ok = false; break; }
       fence_before();
       // T 1: a warp may be a block ahead of another (the next S is there early), so the two S buffers have a barrier each; two blocks ahead it cannot be,
       // since the S after next is issued behind this block's P V
       mbar_arrive(bar(C::PREADY + (T == 1 ? f & 1 : g)));
+      if (unit_done && f + 1 < todo) give_q();                    // the next unit's first S runs while this one's rows are written
 
       // ---- the end of the unit, or of this CTA's piece of it
-      const bool unit_done = use.block + 1 == use.r.blocks;
       if (unit_done || f + 1 == todo) {
-        // a parity says which of two phases has passed only to one who knows that the phase before has: with T 1 this block's S may be there before the
-        // last block's P V (with T 2 it never is)
-        if (T == 1 && f > 0 && !mbar_wait(bar(C::PVFULL + g), (f - 1) & 1, fault, abort_flag)) { ok = false; break; }
         if (!mbar_wait(bar(C::PVFULL + g), f & 1, fault, abort_flag)) { ok = false; break; }
         fence_after();
         if (any && !have) l = NAN;                                // every score -inf (or NaN): what the formula gives
-        const uint32_t unit_begin = share.begin + f - use.block;
-        const bool starts = piece_begin == unit_begin, whole = unit_done && starts;
+        const bool starts = f - piece == use.block, whole = unit_done && starts;
+        const int n = use.row_tile * TILE_ROWS + g * ROWS + t, h = use.hk * args.group + (row.live ? n % args.group : 0);
+        const int64_t token = use.r.first + row.local;
         const float inv = any ? 1.0f / l : 0.0f;
         bf16* dst = args.out.ptr + token * args.out.sn + h * args.out.sh;
         const int64_t at = (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * TILE_ROWS + g * ROWS + t;
         if (warp_live) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             tmem_ld32(o_addr + c * 32, o);
             tmem_wait_ld();
             if (row.live && whole) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) {
-                float x[8];
+              for (int i = 0; i < 32; i += 16) {
+                uint32_t w[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { x[e] = any ? __uint_as_float(o[i + e]) * inv : 0.0f; wrong |= !isfinite(x[e]); }
-                *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+                for (int e = 0; e < 8; ++e) {
+                  const float x = any ? __uint_as_float(o[i + 2 * e]) * inv : 0.0f, y = any ? __uint_as_float(o[i + 2 * e + 1]) * inv : 0.0f;
+                  wrong |= !isfinite(x) || !isfinite(y);
+                  w[e] = pack2_bf16(x, y);
+                }
+                if (args.out_sectors) store32(dst + c * 32 + i, w);
+                else { uint4* d = reinterpret_cast<uint4*>(dst + c * 32 + i); d[0] = make_uint4(w[0], w[1], w[2], w[3]); d[1] = make_uint4(w[4], w[5], w[6], w[7]); }
               }
             } else if (row.live) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(args.work.o + at * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 8) {
+                const uint32_t w[8] = {o[i], o[i + 1], o[i + 2], o[i + 3], o[i + 4], o[i + 5], o[i + 6], o[i + 7]};
+                store32(args.work.o + at * D + c * 32 + i, w);
+              }
             }
           }
           if (row.live && whole && args.lse) args.lse[token * args.heads + h] = any ? m * LN_2 + logf(l) : -INFINITY;
           if (row.live && !whole) args.work.ml[at] = make_float2(have ? m : -INFINITY, l);
         }
         if (!unit_done && starts && tid == 0)
-          args.work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.hk, use.row_tile * TILE_ROWS,
+          args.work.split[blockIdx.x] = SplitUnit{(int)(s_line.of_block(s_line.begin + f - use.block + use.r.blocks - 1) - blockIdx.x) + 1, use.hk, use.row_tile * TILE_ROWS,
                                                     min(TILE_ROWS, use.r.fresh * args.group - use.row_tile * TILE_ROWS), use.r.first};
       }
       use.step(ix, args.group, TILE_ROWS, args.kv_heads, &bad);
@@ -504,7 +558,8 @@ ojc_status launch(const AttnCall& c) {
     attr[c.be->device] = true;
   }
   TcArgs args{rows_view<const bf16>(c.q), rows_view<bf16>(c.out), c.lse, c.ix, c.work, (int)c.a.heads, (int)(c.a.heads / c.a.kv_heads), (int)c.a.kv_heads,
-              c.k->stride[2] < c.k->stride[1], c.v->stride[2] < c.v->stride[1], (int)std::min<int64_t>(c.a.page, KEYS), c.scale, c.be->fault_dev};
+              c.k->stride[2] < c.k->stride[1], c.v->stride[2] < c.v->stride[1],
+              (uintptr_t)c.out->data % 32 == 0 && c.out->stride[0] % 16 == 0 && c.out->stride[1] % 16 == 0, (int)std::min<int64_t>(c.a.page, KEYS), c.scale, c.be->fault_dev};
   CUtensorMap mk, mv;
   OJC_TRY(pages_map(c, &mk, c.k, args.k_heads_inside, args.box_rows));
   OJC_TRY(pages_map(c, &mv, c.v, args.v_heads_inside, args.box_rows));

@@ -349,7 +349,11 @@ def test_attention_in_a_window(be, cached, new, h, hk, d, page, window, bf16, tr
                                                     ([5000], [45], 24, 24, 128, 128), ([3900], [20], 12, 12, 64, 16), ([6000], [12], 8, 8, 96, 16)])
 def test_attention_with_many_key_blocks_to_a_share(be, cached, new, h, hk, d, page):
     """Several units and key blocks to each CTA of every kernel: the rings and barriers go round more than once, warps without rows run beside others."""
-    Case(21, cached, new, h, hk, d, page, True, True).check(be)
+    c = Case(21, cached, new, h, hk, d, page, True, True)
+    out, lse = c.check(be)
+    for _ in range(20):                                    # the order in which warps and copies run differs from run to run, the bits do not
+        again = c.run(be)
+        assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
 
 
 @pytest.mark.parametrize("bf16", [True, False])
