@@ -11,15 +11,16 @@
 
 namespace {
 
-constexpr int PLAN_THREADS = 256, PLAN_TOKENS = 4, PLAN_MAX_BATCH = 24000;
+constexpr int PLAN_THREADS = 256, PLAN_MAX_BATCH = 24000;
 
 // ======================================================================== paged_plan
 // Every CTA scans the lengths for itself (the running sums stay in its shared memory: one launch, no order between CTAs) and then looks up the
 // request of each of its tokens by bisection. A token's page is either entered already (places below the cached length's last page end) or
 // number `first + page - held` of the free pages, so no CTA reads a table entry that another one writes; the token at a page's first place enters it.
+template <int PLAN_TOKENS>
 __global__ void __launch_bounds__(PLAN_THREADS)
 paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restrict__ fresh, const uint32_t* __restrict__ parents, const uint32_t* __restrict__ free_pages,
-                  int64_t n_free, const uint32_t* __restrict__ free_head, uint32_t page, int batch, int64_t width, int64_t tokens, int64_t words,
+                  int64_t n_free, const uint32_t* __restrict__ free_head, uint32_t page, int page_shift, int batch, int64_t width, int64_t tokens, int64_t words,
                   uint32_t* __restrict__ tables, uint32_t* __restrict__ starts, uint32_t* __restrict__ slots, uint32_t* __restrict__ positions,
                   uint32_t* __restrict__ masks, uint32_t* __restrict__ head_out, uint32_t* fault) {
   extern __shared__ uint32_t sm[];
@@ -28,15 +29,17 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   __shared__ unsigned long long w_tok[PLAN_THREADS / 32], w_pg[PLAN_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned long long tok_carry = 0, pg_carry = 0;
+  const uint32_t head32 = *free_head;       // asked for before the lengths' scan
   bool bad = false;
   for (int b0 = 0; b0 < batch; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
     unsigned long long n = 0, g = 0;
     if (b < batch) {
-      const unsigned long long c = cached[b];
-      n = fresh[b];
-      g = (c + n + page - 1) / page - (c + page - 1) / page;
-      bad |= c + n > 0xffffffffull;
+      const uint32_t c = cached[b], k = fresh[b], total = c + k;
+      n = k;
+      bad |= total < c;
+      auto pages = [&](uint32_t x) { const uint32_t q = page_shift >= 0 ? x >> page_shift : x / page; return q + (x != q * page); };
+      g = total < c ? 0 : pages(total) - pages(c);
     }
     unsigned long long tn = n, tg = g;
 #pragma unroll
@@ -59,7 +62,7 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   }
   if (tid == 0) s_start[batch] = (uint32_t)min(tok_carry, (unsigned long long)tokens);
   __syncthreads();
-  const unsigned long long head = *free_head;
+  const unsigned long long head = head32;
   if (blockIdx.x == 0) {
     for (int b = tid; b <= batch; b += PLAN_THREADS) starts[b] = s_start[b];
     if (tid == 0) {
@@ -76,6 +79,9 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
       const int mid = (lo + hi + 1) >> 1;
       if (s_start[mid] <= t0) lo = mid; else hi = mid - 1;
     }
+    int known = -1;                        // the request and the page that the last token looked up: its neighbours mostly share them
+    uint32_t first = 0, c = 0, held = 0, known_page = 0;
+    unsigned long long id = 0;
 #pragma unroll
     for (int u = 0; u < PLAN_TOKENS; ++u) {
       const int64_t t = t0 + u;
@@ -87,18 +93,27 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
         continue;
       }
       while (s_start[lo + 1] <= t) ++lo;   // stops at the latest at the request that holds `last - 1`
-      const uint32_t first = s_start[lo], local = (uint32_t)t - first, c = cached[lo], at = c + local;
-      const uint32_t held = c / page + (c % page != 0), pi = at / page, off = at - pi * page;
-      unsigned long long id = 0xffffffffull;
-      if (pi >= width) bad = true;
-      else if (pi < held) { id = tables[(int64_t)lo * width + pi]; bad |= id == 0xffffffffull; }
-      else {
-        const unsigned long long e = head + s_first[lo] + (pi - held);
-        if (e < (unsigned long long)n_free) {
-          id = free_pages[e];
-          if (off == 0) tables[(int64_t)lo * width + pi] = (uint32_t)id;
+      const bool moved = lo != known;
+      if (moved) {
+        known = lo;
+        first = s_start[lo];
+        c = cached[lo];
+        held = page_shift >= 0 ? c >> page_shift : c / page;
+        held += c != held * page;
+      }
+      const uint32_t local = (uint32_t)t - first, at = c + local;
+      const uint32_t pi = page_shift >= 0 ? at >> page_shift : at / page, off = at - pi * page;
+      if (moved || pi != known_page) {
+        known_page = pi;
+        id = 0xffffffffull;
+        if (pi >= width) bad = true;
+        else if (pi < held) { id = tables[(int64_t)lo * width + pi]; bad |= id == 0xffffffffull; }
+        else {
+          const unsigned long long e = head + s_first[lo] + (pi - held);
+          if (e < (unsigned long long)n_free) id = free_pages[e];
         }
       }
+      if (off == 0 && pi >= held && id != 0xffffffffull) tables[(int64_t)lo * width + pi] = (uint32_t)id;
       const unsigned long long slot = id * page + off;
       if (id != 0xffffffffull) { if (slot < 0xffffffffull) slot4[u] = (uint32_t)slot; else bad = true; }
       // depth and ancestors: indices fall along the chain, so the mask words fill from the token's own downwards
@@ -129,10 +144,15 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
       }
       pos4[u] = c + depth;
     }
-    if (t0 + PLAN_TOKENS <= tokens && ((uintptr_t)slots & 15) == 0 && ((uintptr_t)positions & 15) == 0) {
-      *reinterpret_cast<uint4*>(slots + t0) = make_uint4(slot4[0], slot4[1], slot4[2], slot4[3]);
-      *reinterpret_cast<uint4*>(positions + t0) = make_uint4(pos4[0], pos4[1], pos4[2], pos4[3]);
-    } else {
+    bool stored = false;
+    if constexpr (PLAN_TOKENS == 4) {
+      if (t0 + 4 <= tokens && ((uintptr_t)slots & 15) == 0 && ((uintptr_t)positions & 15) == 0) {
+        *reinterpret_cast<uint4*>(slots + t0) = make_uint4(slot4[0], slot4[1], slot4[2], slot4[3]);
+        *reinterpret_cast<uint4*>(positions + t0) = make_uint4(pos4[0], pos4[1], pos4[2], pos4[3]);
+        stored = true;
+      }
+    }
+    if (!stored) {
       for (int u = 0; u < PLAN_TOKENS && t0 + u < tokens; ++u) { slots[t0 + u] = slot4[u]; positions[t0 + u] = pos4[u]; }
     }
   }
@@ -172,12 +192,12 @@ template <int V> __device__ __forceinline__ void store_v(bf16* p, const float (&
 
 // The rotation of one vector's worth of pairs: V pairs (i, i + half) in the half layout, V / 2 neighbours in the interleaved one. What passes
 // through is an item of its own, moved as it is.
-template <int V, bool INTER> struct Turn {
+template <int V, bool INTER, bool F32_RESULT> struct Turn {
   static constexpr int PAIRS = INTER ? V / 2 : V;
   float c[PAIRS], s[PAIRS];
   __device__ __forceinline__ void set(const ojc_rope& rope, int first_pair, uint32_t position, float sign) {
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) { rope_turn(rope.turns[first_pair + i], position, rope.amplitude, &c[i], &s[i]); s[i] *= sign; }
+    for (int i = 0; i < PAIRS; ++i) { rope_turn<F32_RESULT>(rope.turns[first_pair + i], position, rope.amplitude, &c[i], &s[i]); s[i] *= sign; }
   }
   __device__ __forceinline__ void apply(float (&a)[V], float (&b)[V]) const {   // a alone in the interleaved layout
 #pragma unroll
@@ -192,12 +212,13 @@ template <int V, bool INTER> struct Turn {
 };
 
 // Rotary positions by vectors: a thread forms its pairs' sines and cosines once and goes through `step` heads with them, HEADS at a time so that their
-// loads are in flight together.
+// loads are in flight together (two: 113 us for 32768 x 40 x 128 BF16, 5.9 TB/s; one 129 us, four 146 us with half the warps to an SM).
+// Bound by HBM: every element once in and once out.
 template <class T, int V, bool INTER>
 __global__ void __launch_bounds__(256)
 rope_vector_kernel(const __grid_constant__ ojc_rope rope, const T* x, T* y, const uint32_t* __restrict__ positions, uint32_t rows, uint32_t time, uint32_t pos_rows, int heads, int step,
                    int dim, int64_t xb, int64_t xt, int64_t xh, int64_t yb, int64_t yt, int64_t yh, float sign) {
-  constexpr int HEADS = 4;
+  constexpr int HEADS = 2;
   const uint32_t half = rope.rotary_dim / 2, turned = (INTER ? rope.rotary_dim : half) / V, items = turned + (dim - rope.rotary_dim) / V;
   const uint32_t at = blockIdx.x * 256 + threadIdx.x, row = at / items, item = at % items;
   if (row >= rows) return;
@@ -207,7 +228,7 @@ rope_vector_kernel(const __grid_constant__ ojc_rope rope, const T* x, T* y, cons
   const int e = turns ? (int)(item * V) : (int)(rope.rotary_dim + (item - turned) * V);
   x += b * xb + t * xt + e;
   y += b * yb + t * yt + e;
-  Turn<V, INTER> turn;
+  Turn<V, INTER, std::is_same<T, float>::value> turn;
   if (turns) turn.set(rope, INTER ? e / 2 : e, positions[pos_rows == rows ? row : t], sign);
   for (int h = h0; h < h1; h += HEADS) {
     float u[HEADS][V], v[HEADS][V];
@@ -225,7 +246,8 @@ rope_vector_kernel(const __grid_constant__ ojc_rope rope, const T* x, T* y, cons
   }
 }
 
-// The cache write by vectors: the same items, a rotated key vector (or pair of vectors) with the value's at the same place.
+// The cache write by vectors: the same items, a rotated key vector (or pair of vectors) with the value's at the same place. Bound by HBM: 16384 tokens x
+// 16 x 128 from F32 into BF16 pages 68 us, 5.9 TB/s.
 template <class S, class D, int V, bool INTER>
 __global__ void __launch_bounds__(256)
 paged_kv_write_vector_kernel(const __grid_constant__ ojc_rope rope, PagesView<D> kp, PagesView<D> vp, RowsView<const S> k, RowsView<const S> v, const uint32_t* __restrict__ slots,
@@ -243,7 +265,7 @@ paged_kv_write_vector_kernel(const __grid_constant__ ojc_rope rope, PagesView<D>
   const int e = turns ? (int)(item * V) : (int)(rope.rotary_dim + (item - turned) * V);
   const S *sk = k.ptr + t * k.sn + e, *sv = v.ptr + t * v.sn + e;
   D *dk = kp.ptr + pg * kp.sp + off * kp.st + e, *dv = vp.ptr + pg * vp.sp + off * vp.st + e;
-  Turn<V, INTER> turn;
+  Turn<V, INTER, std::is_same<D, float>::value> turn;
   if (turns) turn.set(rope, INTER ? e / 2 : e, positions[t], 1.0f);
   for (int h = h0; h < h1; h += HEADS) {
     float a[HEADS][V], b[HEADS][V], c[HEADS][V], d[HEADS][V];
@@ -277,9 +299,11 @@ int vector_of(int layout, int rotary, int64_t dim, std::initializer_list<std::pa
   return 0;
 }
 
-// How many heads a thread goes through: all of them when the items alone fill the GPU twice over, fewer when there are few
+// How many heads a thread goes through: with as many threads as the GPU holds at once each has its share of the work, sines and cosines formed once for
+// it. (Twice or four times as many threads: rope 115 against 113 us, write 70 and 78 against 68.)
 int heads_per_thread(const ojc_backend* be, int64_t items, int64_t heads) {
-  return (int)std::max<int64_t>(1, std::min(heads, items * heads / ((int64_t)be->sm_count * 2048)));
+  const int64_t most = std::max<int64_t>(1, std::min(heads, items * heads / ((int64_t)be->sm_count * 2048))), groups = (heads + most - 1) / most;
+  return (int)((heads + groups - 1) / groups);
 }
 
 template <class F> ojc_status by_vector(int v, int layout, F&& f) {
@@ -303,7 +327,7 @@ __global__ void rope_kernel(const __grid_constant__ ojc_rope rope, const T* x, T
     T* py = y + b * yb + t * yt + h * yh;
     if (e >= half) { py[rope.rotary_dim + e - half] = px[rope.rotary_dim + e - half]; continue; }
     float c, s;
-    rope_turn(rope.turns[e], positions[row % pos_rows], rope.amplitude, &c, &s);
+    rope_turn<std::is_same<T, float>::value>(rope.turns[e], positions[row % pos_rows], rope.amplitude, &c, &s);
     s *= sign;
     const int i0 = rope.layout ? 2 * e : e, i1 = rope.layout ? 2 * e + 1 : e + half;
     const float u = ldf(px, i0), v = ldf(px, i1);
@@ -334,7 +358,7 @@ __global__ void paged_kv_write_kernel(const __grid_constant__ ojc_rope rope, boo
       const bool second = rope.layout ? (e & 1) : e >= half;
       const float other = ldf(pk, rope.layout ? e ^ 1 : second ? e - half : e + half);
       float c, s;
-      rope_turn(rope.turns[pair], positions[t], rope.amplitude, &c, &s);
+      rope_turn<std::is_same<D, float>::value>(rope.turns[pair], positions[t], rope.amplitude, &c, &s);
       a = second ? turned_second(other, a, c, s) : turned_first(a, other, c, s);
     }
     stf(kp.ptr + pg * kp.sp + off * kp.st + h * kp.sh, e, a);
@@ -470,14 +494,17 @@ ojc_status ojc_paged_plan(ojc_backend* be, const ojc_tensor* cached_lens, const 
   const size_t smem = (size_t)(2 * batch + 1) * 4;
   static PerDeviceFlag attr;
   if (smem > 48 * 1024 - 256 && !attr[be->device]) {
-    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
+    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
+    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
     attr[be->device] = true;
   }
-  const int64_t per_cta = PLAN_THREADS * PLAN_TOKENS;
+  // a token to a thread while that gives every SM a few CTAs at most (trees' chains of parents then run side by side), else four and 16-byte stores
+  const int per_thread = tokens <= (int64_t)be->sm_count * PLAN_THREADS * 4 ? 1 : 4;
+  const int64_t per_cta = PLAN_THREADS * per_thread;
   const unsigned grid = (unsigned)std::min<int64_t>((tokens + per_cta - 1) / per_cta, (int64_t)be->sm_count * 4);
-  paged_plan_kernel<<<grid, PLAN_THREADS, smem, be->stream>>>(
+  (per_thread == 1 ? paged_plan_kernel<1> : paged_plan_kernel<4>)<<<grid, PLAN_THREADS, smem, be->stream>>>(
       (const uint32_t*)cached_lens->data, (const uint32_t*)new_lens->data, parents ? (const uint32_t*)parents->data : nullptr, (const uint32_t*)free_pages->data,
-      free_pages->shape[0], (const uint32_t*)free_head->data, (uint32_t)page_size, (int)batch, width, tokens, words, (uint32_t*)block_tables->data, (uint32_t*)starts->data,
+      free_pages->shape[0], (const uint32_t*)free_head->data, (uint32_t)page_size, (page_size & (page_size - 1)) ? -1 : __builtin_ctzll((unsigned long long)page_size), (int)batch, width, tokens, words, (uint32_t*)block_tables->data, (uint32_t*)starts->data,
       (uint32_t*)slots->data, (uint32_t*)positions->data, masks ? (uint32_t*)masks->data : nullptr, (uint32_t*)free_head_out->data, be->fault_dev);
   OJC_LAUNCHED(be, op);
   return OJC_OK;

@@ -22,10 +22,14 @@ inline RowsView<P> rows_view(const ojc_tensor* t) { return RowsView<P>{(P*)t->da
 
 #ifdef __CUDACC__
 // Rotation of a pair: the angle is position x frequency with the frequency in 2^-64 turns, so the product modulo 2^64 IS the angle's fraction of a
-// turn, exact to position x 2^-64 however far the position; its upper half as a signed integer is the angle / pi in [-1, 1) x 2^31.
+// turn, exact to position x 2^-64 however far the position; its upper half as a signed integer is the angle / pi in [-1, 1) x 2^31. What is rounded to
+// BF16 (2^-8) takes the special-function unit's sine and cosine, whose absolute error on [-pi, pi] is about 2^-21; F32 results take sincospif.
+template <bool F32_RESULT>
 __device__ __forceinline__ void rope_turn(uint64_t turns, uint32_t position, float amplitude, float* c, float* s) {
   const uint64_t t = turns * position;
-  sincospif((float)(int32_t)(uint32_t)(t >> 32) * 4.656612873077393e-10f, s, c);
+  const float half_turns = (float)(int32_t)(uint32_t)(t >> 32) * 4.656612873077393e-10f;
+  if (F32_RESULT) sincospif(half_turns, s, c);
+  else __sincosf(half_turns * 3.14159265358979f, s, c);
   *c = __fmul_rn(*c, amplitude);
   *s = __fmul_rn(*s, amplitude);
 }
