@@ -145,9 +145,11 @@ template <class T, int D, int MW> struct TileShape {
   static constexpr int STAGE = BLOCK_KEYS * (K_PITCH + V_PITCH) * (int)sizeof(T);
   static constexpr bool Q_IN_REGS = std::is_same<T, bf16>::value && D <= 128;
   static constexpr int JOINT = MW < TILE_WARPS ? 16 * (D + 2) * 4 : 0, OFFSETS = TILE_WARPS * 32 * 8, Q_TILE = Q_IN_REGS ? 0 : 16 * MW * K_PITCH * (int)sizeof(T);
-  static constexpr int STAGES = 3 * STAGE + JOINT + OFFSETS + Q_TILE <= 226 * 1024 ? 3 : 2;          // what an SM holds
-  static constexpr int SMEM = STAGES * STAGE + JOINT + OFFSETS + Q_TILE;
-  static constexpr int CTAS_PER_SM = SMEM <= 112 * 1024 + 512 ? 2 : 1;
+  // what an SM holds: two CTAs of three stages, or of two, or one CTA
+  static constexpr int REST = JOINT + OFFSETS + Q_TILE, HALF_SM = 112 * 1024 + 512;
+  static constexpr int STAGES = 3 * STAGE + REST <= HALF_SM ? 3 : 2 * STAGE + REST <= HALF_SM ? 2 : 3 * STAGE + REST <= 226 * 1024 ? 3 : 2;
+  static constexpr int SMEM = STAGES * STAGE + REST;
+  static constexpr int CTAS_PER_SM = SMEM <= HALF_SM ? 2 : 1;
 };
 
 template <class T, int D, int MW>
@@ -241,10 +243,13 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
       live[x] = r < use.r.fresh * group;
       local[x] = live[x] ? r / group : 0;
       const int64_t t = use.r.first + local[x];
-      const uint32_t place = ix.positions ? ix.positions[t] : use.r.cached + (uint32_t)local[x];
-      from[x] = ix.window > 0 && place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
-      if (live[x] && ix.window > 0 && place < use.r.cached) bad = true;
-      if (live[x]) from_most = max(from_most, from[x]);
+      from[x] = 0;
+      if (ix.window > 0) {
+        const uint32_t place = ix.positions ? ix.positions[t] : use.r.cached + (uint32_t)local[x];
+        from[x] = place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
+        if (live[x] && place < use.r.cached) bad = true;
+        if (live[x]) from_most = max(from_most, from[x]);
+      }
       m[x] = -INFINITY; l[x] = 0.0f; any[x] = false;
       if (S::Q_IN_REGS) {
         const uint32_t* p = reinterpret_cast<const uint32_t*>(q.ptr + t * q.sn + (int64_t)(hk * group + (live[x] ? r % group : 0)) * q.sh);
@@ -253,17 +258,15 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
       }
     }
     if (ix.window > 0) from_most = __reduce_max_sync(0xffffffffu, from_most);
-    if (!S::Q_IN_REGS) {
+    if (!S::Q_IN_REGS) {                                                                                 // by copies: the first unit's ride with the first block's
       __syncthreads();
       for (int i = tid; i < TILE_ROWS * CHUNKS; i += TILE_WARPS * 32) {
         const int r = i / CHUNKS, c = i % CHUNKS, g = row_tile * TILE_ROWS + r;
-        const bool has = g < use.r.fresh * group;
-        const T* p = q.ptr + (int64_t)(use.r.first + (has ? g / group : 0)) * q.sn + (int64_t)(hk * group + (has ? g % group : 0)) * q.sh + c * PER;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (has) v = *reinterpret_cast<const uint4*>(p);
-        *reinterpret_cast<uint4*>(q_tile + r * S::K_PITCH + c * PER) = v;
+        T* dst = q_tile + r * S::K_PITCH + c * PER;
+        if (g < use.r.fresh * group) copy16(smem_addr(dst), q.ptr + (int64_t)(use.r.first + g / group) * q.sn + (int64_t)(hk * group + g % group) * q.sh + c * PER);
+        else *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
       }
-      __syncthreads();
+      if (at != begin) { copies_commit(); copies_wait<0>(); __syncthreads(); }
     }
 #pragma unroll
     for (int n = 0; n < OT; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
@@ -287,7 +290,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     const int row_tile = use.row_tile, hk = use.hk;
 
     copies_wait<STAGES - 2>();
-    if (MW == 1) __syncwarp(); else __syncthreads();
+    if (MW == 1 && (S::Q_IN_REGS || f > 0)) __syncwarp(); else __syncthreads();
     {                                                                                                   // the stage that the last block left
       const int next = f + STAGES - 1;
       if (next < todo) { copy_block(stage == 0 ? STAGES - 1 : stage - 1, next_place); if (next + 1 < todo) next_place = look_up(); }
@@ -318,6 +321,11 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         }
       }
     } else {
+      // with few tiles to a warp the three products of a step have sums of their own: a third of the chain of dependent products
+      constexpr bool APART = NT <= 4;
+      float s1[APART ? NT : 1][4], s2[APART ? NT : 1][4];
+#pragma unroll
+      for (int n = 0; n < (APART ? NT : 1); ++n) { s1[n][0] = s1[n][1] = s1[n][2] = s1[n][3] = 0.0f; s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f; }
       const float* qa = reinterpret_cast<const float*>(q_tile) + (16 * mw + quad) * S::K_PITCH + pair;
       const float* ka = reinterpret_cast<const float*>(kt) + quad * S::K_PITCH + pair;
 #pragma unroll 4
@@ -329,9 +337,16 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         for (int n = 0; n < NT; ++n) {
           uint32_t bh0, bl0, bh1, bl1;
           split_tf32(ka[n * 8 * S::K_PITCH + 8 * k], &bh0, &bl0); split_tf32(ka[n * 8 * S::K_PITCH + 8 * k + 4], &bh1, &bl1);
-          mma_tf32(s[n], al, bh0, bh1);
-          mma_tf32(s[n], ah, bl0, bl1);
+          mma_tf32(APART ? s1[APART ? n : 0] : s[n], al, bh0, bh1);
+          mma_tf32(APART ? s2[APART ? n : 0] : s[n], ah, bl0, bl1);
           mma_tf32(s[n], ah, bh0, bh1);
+        }
+      }
+      if (APART) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] += s1[APART ? n : 0][e] + s2[APART ? n : 0][e];
         }
       }
     }
