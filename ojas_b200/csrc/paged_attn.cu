@@ -106,13 +106,13 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 }
 
 // ======================================================================== tiles on the tensor cores
-// Row tiles of 16 * MW rows, key blocks of 64 (paged_attn.cuh has the line of work).
+// Row tiles of 16 * MW rows, key blocks of 64 or 128 (paged_attn.cuh has the line of work).
 //
 // What bounds it: the cache's bytes for few rows. Four warps to a CTA, two CTAs to an SM, three stages of 64 keys each, rows fetched by 16-byte asynchronous
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
 // Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
-constexpr int BLOCK_KEYS = 64, TILE_WARPS = 4;
+constexpr int TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -141,10 +141,12 @@ __device__ __forceinline__ float quad_max(float v) { v = fmaxf(v, __shfl_xor_syn
 __device__ __forceinline__ float quad_sum(float v) { v += __shfl_xor_sync(0xffffffffu, v, 1); return v + __shfl_xor_sync(0xffffffffu, v, 2); }
 
 template <class T, int D, int MW> struct TileShape {
+  // keys to a block: 64, or 128 where rows are short and a warp would have little to do with 16 of them (one row tile, BF16, 64 columns)
+  static constexpr int KEYS = std::is_same<T, bf16>::value && D == 64 && MW < 4 ? 128 : 64, WARP_KEYS = KEYS / TILE_WARPS;
   static constexpr int K_PITCH = std::is_same<T, float>::value ? D + 4 : D + 8, V_PITCH = D + 8;   // elements: odd multiples of 16 bytes (ldmatrix), or 4 and 8 banks a row (F32 fragments)
-  static constexpr int STAGE = BLOCK_KEYS * (K_PITCH + V_PITCH) * (int)sizeof(T);
+  static constexpr int STAGE = KEYS * (K_PITCH + V_PITCH) * (int)sizeof(T);
   static constexpr bool Q_IN_REGS = std::is_same<T, bf16>::value && D <= 128;
-  static constexpr int JOINT = MW < TILE_WARPS ? 16 * (D + 2) * 4 : 0, OFFSETS = TILE_WARPS * 32 * 8, Q_TILE = Q_IN_REGS ? 0 : 16 * MW * K_PITCH * (int)sizeof(T);
+  static constexpr int JOINT = MW < TILE_WARPS ? 16 * (D + 2) * 4 : 0, OFFSETS = 2 * KEYS * 8, Q_TILE = Q_IN_REGS ? 0 : 16 * MW * K_PITCH * (int)sizeof(T);
   // what an SM holds: two CTAs of three stages, or of two, or one CTA
   static constexpr int REST = JOINT + OFFSETS + Q_TILE, HALF_SM = 112 * 1024 + 512;
   static constexpr int STAGES = 3 * STAGE + REST <= HALF_SM ? 3 : 2 * STAGE + REST <= HALF_SM ? 2 : 3 * STAGE + REST <= 226 * 1024 ? 3 : 2;
@@ -159,13 +161,14 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   using S = TileShape<T, D, MW>;
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr int STAGES = S::STAGES;
+  constexpr int BLOCK_KEYS = S::KEYS, WARP_KEYS = S::WARP_KEYS;                                           // WARP_KEYS: those that a warp fetches
   constexpr int KW = TILE_WARPS / MW, KEYS = BLOCK_KEYS / KW, NT = KEYS / 8, OT = D / 8, TILE_ROWS = 16 * MW;
   constexpr int CHUNKS = D * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
   constexpr int KSTEP = F32 ? 8 : 16, KSTEPS = D / KSTEP;
   extern __shared__ __align__(128) uint8_t raw[];
   float* joint = reinterpret_cast<float*>(raw + STAGES * S::STAGE);                                   // [16][D] and [16] (m, l): the warps' outputs meet here
   uint64_t* rows_at = reinterpret_cast<uint64_t*>(raw + STAGES * S::STAGE + S::JOINT);
-  T* q_tile = reinterpret_cast<T*>(rows_at + TILE_WARPS * 32);                                          // only without Q_IN_REGS
+  T* q_tile = reinterpret_cast<T*>(rows_at + 2 * BLOCK_KEYS);                                          // only without Q_IN_REGS
   __shared__ ShareScratch s_share;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, mw = warp % MW, kw = warp / MW, quad = lane >> 2, pair = lane & 3;
   bool bad = false, wrong = false;
@@ -180,15 +183,15 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   Cursor<BLOCK_KEYS> use = share.at;
   Cursor<BLOCK_KEYS> ahead = use;                                                                                   // the block whose pages are looked up next
 
-  // ---- copies: warp w fetches keys 16 w .. 16 w + 15 of a block; lane l looks up key l's row of K, lane 16 + l its row of V. Places behind the last
-  // one repeat it: what lies there is masked like any place that is not seen.
+  // ---- copies: warp w fetches WARP_KEYS keys of a block from number w * WARP_KEYS on; with 16, lane l looks up key l's row of K and lane 16 + l its row of V,
+  // with 32 a lane does both. Places behind the last one repeat it: what lies there is masked like any place that is not seen.
   const PagesView<const T>& mine = lane < 16 ? kp : vp;
   const char* const mine_ptr = (const char*)mine.ptr;
   const int64_t mine_sp = mine.sp * (int)sizeof(T), mine_st = mine.st * (int)sizeof(T), mine_sh = mine.sh * (int)sizeof(T);
   struct Place { uint32_t id, off; int hk; };
   auto look_up = [&]() {
     Place p;
-    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + 16 * warp + (lane & 15)), last);
+    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + WARP_KEYS * warp + lane % WARP_KEYS), last);
     const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
     p.off = j - pi * ix.page;
     p.id = ix.tables[(int64_t)ahead.b * ix.width + pi];
@@ -196,12 +199,16 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
     ahead.step(ix, group, TILE_ROWS, kv_heads, &bad);
     return p;
   };
-  uint64_t* my_rows = rows_at + warp * 32;
-  const uint32_t k_base = smem_addr(raw) + (16 * warp + lane / CHUNKS) * S::K_PITCH * (int)sizeof(T) + (lane % CHUNKS) * 16;
-  const uint32_t v_base = smem_addr(raw) + (BLOCK_KEYS * S::K_PITCH + (16 * warp + lane / CHUNKS) * S::V_PITCH) * (int)sizeof(T) + (lane % CHUNKS) * 16;
+  uint64_t* my_rows = rows_at + warp * 2 * WARP_KEYS;                                                   // K's, then V's
+  const uint32_t k_base = smem_addr(raw) + (WARP_KEYS * warp + lane / CHUNKS) * S::K_PITCH * (int)sizeof(T) + (lane % CHUNKS) * 16;
+  const uint32_t v_base = smem_addr(raw) + (BLOCK_KEYS * S::K_PITCH + (WARP_KEYS * warp + lane / CHUNKS) * S::V_PITCH) * (int)sizeof(T) + (lane % CHUNKS) * 16;
   auto copy_block = [&](int stage, Place p) {
     if (p.id >= ix.pages) { bad = true; p.id = 0; }
-    my_rows[lane] = (uint64_t)(mine_ptr + (int64_t)p.id * mine_sp + (int64_t)p.off * mine_st + (int64_t)p.hk * mine_sh);
+    if (WARP_KEYS == 16) my_rows[lane] = (uint64_t)(mine_ptr + (int64_t)p.id * mine_sp + (int64_t)p.off * mine_st + (int64_t)p.hk * mine_sh);
+    else {
+      my_rows[lane] = (uint64_t)(kp.ptr + p.id * kp.sp + p.off * kp.st + p.hk * kp.sh);
+      my_rows[32 + lane] = (uint64_t)(vp.ptr + p.id * vp.sp + p.off * vp.st + p.hk * vp.sh);
+    }
     __syncwarp();
     const uint32_t ka = k_base + stage * S::STAGE, va = v_base + stage * S::STAGE;
     if constexpr (32 % CHUNKS == 0) {                                                                   // a lane keeps its column of 16 bytes
@@ -209,17 +216,17 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
       const uint64_t* at = my_rows + lane / CHUNKS;
       const int c = (lane % CHUNKS) * 16;
 #pragma unroll
-      for (int i = 0; i < 16 / ROWS; ++i) copy16(ka + i * ROWS * S::K_PITCH * (int)sizeof(T), (const char*)at[i * ROWS] + c);
+      for (int i = 0; i < WARP_KEYS / ROWS; ++i) copy16(ka + i * ROWS * S::K_PITCH * (int)sizeof(T), (const char*)at[i * ROWS] + c);
 #pragma unroll
-      for (int i = 0; i < 16 / ROWS; ++i) copy16(va + i * ROWS * S::V_PITCH * (int)sizeof(T), (const char*)at[16 + i * ROWS] + c);
+      for (int i = 0; i < WARP_KEYS / ROWS; ++i) copy16(va + i * ROWS * S::V_PITCH * (int)sizeof(T), (const char*)at[WARP_KEYS + i * ROWS] + c);
     } else {
-      const uint32_t kw0 = smem_addr(raw) + stage * S::STAGE + 16 * warp * S::K_PITCH * (int)sizeof(T);
-      const uint32_t vw0 = smem_addr(raw) + stage * S::STAGE + (BLOCK_KEYS * S::K_PITCH + 16 * warp * S::V_PITCH) * (int)sizeof(T);
+      const uint32_t kw0 = smem_addr(raw) + stage * S::STAGE + WARP_KEYS * warp * S::K_PITCH * (int)sizeof(T);
+      const uint32_t vw0 = smem_addr(raw) + stage * S::STAGE + (BLOCK_KEYS * S::K_PITCH + WARP_KEYS * warp * S::V_PITCH) * (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < CHUNKS / 2; ++i) {
+      for (int i = 0; i < CHUNKS * WARP_KEYS / 32; ++i) {
         const int n = lane + 32 * i, row = n / CHUNKS, c = n % CHUNKS * 16;
         copy16(kw0 + row * S::K_PITCH * (int)sizeof(T) + c, (const char*)my_rows[row] + c);
-        copy16(vw0 + row * S::V_PITCH * (int)sizeof(T) + c, (const char*)my_rows[16 + row] + c);
+        copy16(vw0 + row * S::V_PITCH * (int)sizeof(T) + c, (const char*)my_rows[WARP_KEYS + row] + c);
       }
     }
     __syncwarp();
