@@ -517,3 +517,78 @@ def test_a_decoding_loop_over_pages(be, bf16):
             cached[b] += len(kept)
         head = u32(be, [int(p.free_head.numpy()[0])])    # pages of dropped drafts stay in their request's table
     be.sync()
+
+
+def test_a_pass_in_a_graph_replays_with_new_lengths_and_workspaces(be):
+    """Plan, rotation, write and attention captured once from the backend's stream; replayed after the lengths, the inputs and the pages' contents changed,
+    with eager calls (which may grow the library's own workspace) between. Without a workspace of its own the attention refuses to be captured."""
+    from cuda.bindings import runtime as rt
+    from ojas_b200 import DType, OjasError, RopeSpec
+    rng = np.random.default_rng(30)
+    h, hk, d, page, pool, width, capacity = 8, 2, 64, 16, 80, 40, 24
+
+    def ok(r):
+        assert r[0] == rt.cudaError_t.cudaSuccess, r[0]
+        return r[1] if len(r) > 1 else None
+    plan = be.rope_plan(RopeSpec(d))
+    cached, new, head = u32(be, [0, 0]), u32(be, [1, 1]), u32(be, [0])
+    free, tables = u32(be, rng.permutation(pool)), u32(be, np.full((2, width), NONE))
+    parents = u32(be, np.full(capacity, NONE))
+    q, k, v = (be.zeros((capacity, n, d), DType.F32) for n in (h, hk, hk))
+    qb, out, lse = be.zeros((capacity, h, d), DType.F32), be.zeros((capacity, h, d), DType.F32), be.zeros((capacity, h))
+    kp, vp = be.zeros((pool, page, hk, d)), be.zeros((pool, page, hk, d))
+    work = be.paged_attention_workspace(q, kp)
+    keep = {n: be.empty(s, DType.U32) for n, s in dict(starts=(3,), slots=(capacity,), positions=(capacity,), masks=(capacity, 1), free_head_out=(1,)).items()}
+
+    def one_pass(workspace):
+        p = be.paged_plan(cached, new, free, head, tables, page, parents=parents, **keep)
+        be.rope_forward(q, p.positions, plan, out=qb)
+        be.paged_kv_write(kp, vp, k, v, p.slots, rope=plan, positions=p.positions)
+        be.paged_attention_forward(qb, kp, vp, tables, cached, p.starts, masks=p.masks, positions=p.positions, out=out, lse=lse, workspace=workspace)
+    one_pass(work)                                       # what is set up once happens outside the capture
+    be.sync()
+    stream = be.stream()
+    mode = rt.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal
+    ok(rt.cudaStreamBeginCapture(stream, mode))
+    with pytest.raises(OjasError) as e:
+        one_pass(None)
+    assert e.value.kind == "Unsupported"
+    ok(rt.cudaGraphDestroy(ok(rt.cudaStreamEndCapture(stream))))
+    ok(rt.cudaStreamBeginCapture(stream, mode))
+    one_pass(work)
+    graph = ok(rt.cudaStreamEndCapture(stream))
+    run = ok(rt.cudaGraphInstantiate(graph, 0))
+    import ctypes as C
+    from ojas_b200._lib import lib
+    from ojas_b200.backend import _check
+
+    def put(t, a):
+        a = np.ascontiguousarray(a, np.float32 if t.dtype == DType.F32 else np.uint32)
+        _check(lib.ojc_upload(be._handle, C.c_void_p(t.ptr), C.c_void_p(a.ctypes.data), C.c_uint64(a.nbytes)))
+    for lens, news in (([0, 0], [3, 17]), ([100, 300], [12, 1]), ([16, 0], [20, 0]), ([500, 511], [7, 9])):
+        par = np.concatenate([tree_parents(rng, news), np.zeros(capacity - sum(news), np.int64)])
+        qs, ks, vs = (rng.standard_normal((capacity, n, d)).astype(np.float32) for n in (h, hk, hk))
+        pages_k, pages_v = (rng.standard_normal((pool, page, hk, d)).astype(np.float32) for _ in range(2))
+        order = rng.permutation(pool)
+        held = [-(-c // page) for c in lens]
+        tab = np.full((2, width), NONE, np.int64)
+        tab[0, :held[0]], tab[1, :held[1]] = order[:held[0]], order[held[0]:sum(held)]
+        rest = np.concatenate([order[sum(held):], np.full(sum(held), 7)])
+        for t, a in ((cached, lens), (new, news), (parents, par), (q, qs), (k, ks), (v, vs), (kp, pages_k), (vp, pages_v), (tables, tab), (free, rest)):
+            put(t, np.asarray(a))
+        put(out, np.full((capacity, h, d), 7.0)); put(lse, np.full((capacity, h), 7.0))
+        ok(rt.cudaGraphLaunch(run, stream))
+        got, got_lse, got_k = out.numpy(), lse.numpy(), kp.numpy()
+        be.sync()
+        for t, a in ((kp, pages_k), (vp, pages_v), (tables, tab)):
+            put(t, np.asarray(a))
+        put(out, np.full((capacity, h, d), 7.0)); put(lse, np.full((capacity, h), 7.0))
+        one_pass(None)                                   # eager, in the library's own workspace
+        assert np.array_equal(out.numpy(), got) and np.array_equal(lse.numpy(), got_lse) and np.array_equal(kp.numpy(), got_k)
+        assert np.all(got[sum(news):] == 7.0)
+        starts = keep["starts"].numpy()
+        want, _, tol, _ = ref.attention(qb.numpy()[:sum(news)], got_k, vp.numpy(), tables.numpy(), np.array(lens), starts, keep["masks"].numpy(), keep["positions"].numpy(), None, HALF_F32, 0.0)
+        assert np.all(np.abs(got[:sum(news)] - want) <= tol)
+        be.linear_forward(be.upload(rng.standard_normal((64, 64)).astype(np.float32)), be.upload(rng.standard_normal((64, 64)).astype(np.float32)))
+    ok(rt.cudaGraphExecDestroy(run)); ok(rt.cudaGraphDestroy(graph))
+    be.sync()
