@@ -732,7 +732,7 @@ ojc_status tiles_launch(const AttnCall& c) {
     attr[c.be->device] = true;
   }
   static_assert(S::CTAS_PER_SM * REDUCE_SMS <= MAX_SHARES && S::CTAS_PER_SM * REDUCE_SMS * 16 * MW <= MAX_SHARE_ROWS, "workspace");
-  const unsigned ctas = S::CTAS_PER_SM * REDUCE_SMS;
+  const unsigned ctas = attn_ctas(c, S::CTAS_PER_SM * REDUCE_SMS, 16 * MW, S::KEYS);
   const int group = (int)(c.a.heads / c.a.kv_heads);
   // queued while the kernel before still runs; it waits for that one's end before it looks at memory
   cudaLaunchAttribute early;

@@ -33,6 +33,12 @@ struct AttnCall {
   const ojc_tensor *q, *k, *v; ojc_tensor* out; float* lse;
   PassIndex ix; AttnDims a; float scale; TileWork work;
 };
+// CTAs to launch: one wave, or fewer where the longest requests that the tables allow would not give each the two blocks that a share has at least
+inline unsigned attn_ctas(const AttnCall& c, int wave, int tile_rows, int keys) {
+  const int64_t rows = c.a.tokens * (c.a.heads / c.a.kv_heads), tiles = (rows + tile_rows - 1) / tile_rows + c.ix.batch;
+  const double most = (double)tiles * (double)c.a.kv_heads * (double)(c.ix.width * c.ix.page / keys + 1);
+  return most / 2 + 1 < wave ? (unsigned)(most / 2 + 1) : (unsigned)wave;
+}
 // The joining kernel behind one that ran `shares` CTAs with tiles of `tile_rows` rows
 ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows);
 // tcgen05 / TMEM form with one or two tiles of 128 rows (BF16, head_dim 64 or 128, pages that tile 128 keys)

@@ -568,7 +568,8 @@ ojc_status launch(const AttnCall& c) {
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(REDUCE_SMS);
+  const unsigned ctas = attn_ctas(c, REDUCE_SMS, ROWS * T, KEYS);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = c.be->stream;
@@ -576,7 +577,7 @@ ojc_status launch(const AttnCall& c) {
   cfg.numAttrs = 1;
   OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tcgen05_kernel<D, T>, mk, mv, args), c.op);
   c.be->launches++;
-  return paged_attention_join(c, REDUCE_SMS, ROWS * T);
+  return paged_attention_join(c, ctas, ROWS * T);
 }
 
 }  // namespace

@@ -592,3 +592,13 @@ def test_a_pass_in_a_graph_replays_with_new_lengths_and_workspaces(be):
         be.linear_forward(be.upload(rng.standard_normal((64, 64)).astype(np.float32)), be.upload(rng.standard_normal((64, 64)).astype(np.float32)))
     ok(rt.cudaGraphExecDestroy(run)); ok(rt.cudaGraphDestroy(graph))
     be.sync()
+
+
+@pytest.mark.parametrize("cached,h,hk,d,new", [(60000, 4, 1, 128, 1), (30000, 2, 2, 64, 3), (40000, 16, 1, 64, 5), (25000, 8, 1, 96, 2)])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_long_sequence_in_many_pieces(be, cached, h, hk, d, new, bf16):
+    """One unit over most of the GPU: many pieces to join; twice with the same bits."""
+    c = Case(32, [cached], [new], h, hk, d, 64, True, bf16)
+    out, lse = c.check(be, workspace=True)
+    again = c.run(be)
+    assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
