@@ -37,7 +37,7 @@ struct AttnCall {
 inline unsigned attn_ctas(const AttnCall& c, int wave, int tile_rows, int keys) {
   const int64_t rows = c.a.tokens * (c.a.heads / c.a.kv_heads), tiles = (rows + tile_rows - 1) / tile_rows + c.ix.batch;
   const double most = (double)tiles * (double)c.a.kv_heads * (double)(c.ix.width * c.ix.page / keys + 1);
-  return most / 2 + 1 < wave ? (unsigned)(most / 2 + 1) : (unsigned)wave;
+  return most < wave ? (unsigned)most : (unsigned)wave;
 }
 // The joining kernel behind one that ran `shares` CTAs with tiles of `tile_rows` rows
 ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows);
@@ -126,7 +126,7 @@ __device__ __forceinline__ bool find_share(const PassIndex& ix, int group, int t
     const uint32_t sum = scan(n, &upto);
     if ((unsigned long long)total + sum < 1ull << 31) total += sum; else *bad = true;
   }
-  out->ctas = min(gridDim.x, (total + 1) / 2);                   // at least two blocks each
+  out->ctas = min(gridDim.x, total);
   if (blockIdx.x >= out->ctas) return false;
   out->share = total / out->ctas;
   out->longer = total - out->share * out->ctas;
