@@ -751,14 +751,15 @@ ojc_status tiles_launch(const AttnCall& c) {
   return paged_attention_join(c, ctas, 16 * MW);
 }
 
-#ifndef ROWS_TC
-#define ROWS_TC 16
-#endif
 template <class T, int D>
 ojc_status tiles_by_rows(const AttnCall& c) {
   // rows of a KV head in a request of average length: what the host knows without a readback
   const int64_t rows = (c.a.tokens + c.ix.batch - 1) / c.ix.batch * (c.a.heads / c.a.kv_heads);
-  if ((D == 64 || D == 128) && rows > ROWS_TC && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
+  // More than 32 rows: tcgen05 (48 drafts over 4000 cached, 16 heads of 128: 55 us against 76; 100 drafts 61 against 117). 17 to 32 rows: its tiles of 128 rows
+  // are mostly empty and the tiles here are ahead (31 drafts: 51 against 57 us at 1000 cached, 60 against 62 at 4000), except over long contexts, where the
+  // page copies by boxes count (20 rows over 131 thousand: 107 against 123 us).
+  const bool wide = rows > 32 || (rows > 16 && c.ix.width * c.ix.page >= 32768);
+  if ((D == 64 || D == 128) && wide && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
   if (rows <= 16) return tiles_launch<T, D, 1>(c);
   if (rows <= 32) return tiles_launch<T, D, 2>(c);
   return tiles_launch<T, D, 4>(c);
