@@ -388,6 +388,7 @@ ojc_status rope_run(ojc_backend* be, const char* op, const ojc_rope* rope, const
   OJC_TRY(rope_check(op, rope, dim));
   const int64_t np = numel(positions);
   if (np != rows && !(r == 4 && np == time)) return ojc_fail(OJC_ERR_SHAPE, op, "positions hold one entry per token, or per time step of a rank-4 tensor");
+  OJC_CUDA(be, cudaSetDevice(be->device), op);   // the caller's current device may be another backend's
   const int64_t xb = r == 4 ? x->stride[0] : 0, yb = r == 4 ? y->stride[0] : 0;
   return dispatch_float(op, x->dtype, [&](auto t) {
     using T = decltype(t);
@@ -491,6 +492,7 @@ ojc_status ojc_paged_plan(ojc_backend* be, const ojc_tensor* cached_lens, const 
   if (tokens > INT32_MAX || width > INT32_MAX) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "extent out of range");
   if (page_size < 1 || page_size > (1 << 24)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "page_size must be in 1..=2^24");
   if (free_head_out->data == free_head->data) return ojc_fail(OJC_ERR_SHAPE, op, "free_head_out must be another tensor than free_head");
+  OJC_CUDA(be, cudaSetDevice(be->device), op);
   const size_t smem = (size_t)(2 * batch + 1) * 4;
   static PerDeviceFlag attr;
   if (smem > 48 * 1024 - 256 && !attr[be->device]) {
@@ -525,6 +527,7 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
   if (page > (1 << 24) || heads > INT32_MAX || dim > INT32_MAX || pages > (int64_t)OJC_NONE / page) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "slot numbers do not fit U32");
   OJC_TRY(u32_vector(op, "slots", slots, tokens));
   if (rope) { OJC_TRY(rope_check(op, rope, dim)); OJC_TRY(u32_vector(op, "positions", positions, tokens)); }
+  OJC_CUDA(be, cudaSetDevice(be->device), op);
   return dispatch_float(op, k->dtype, [&](auto s) {
     using S = decltype(s);
     return dispatch_float(op, k_pages->dtype, [&](auto d) {

@@ -29,7 +29,7 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * nwarps + warp, t = row / heads;
   const int h = (int)(row % heads), hk = h / group;
-  if (t >= ix.tokens || t >= ix.starts[ix.batch]) return;
+  if (t >= ix.tokens || t >= ix.starts[ix.batch] || t < ix.starts[0]) return;
   const int b = request_of(ix.starts, ix.batch, (uint32_t)t);
   const uint32_t first = ix.starts[b], end = ix.starts[b + 1], local = (uint32_t)t - first;
   const int64_t cached = ix.cached[b], room = ix.width * ix.page;
@@ -147,11 +147,14 @@ template <class T, int D, int MW> struct TileShape {
   static constexpr int STAGE = KEYS * (K_PITCH + V_PITCH) * (int)sizeof(T);
   static constexpr bool Q_IN_REGS = std::is_same<T, bf16>::value && D <= 128;
   static constexpr int JOINT = MW < TILE_WARPS ? 16 * (D + 2) * 4 : 0, OFFSETS = 2 * KEYS * 8, Q_TILE = Q_IN_REGS ? 0 : 16 * MW * K_PITCH * (int)sizeof(T);
-  // what an SM holds: two CTAs of three stages, or of two, or one CTA
+  // What else an SM holds: two CTAs of three stages, or of two, or one CTA.
   static constexpr int REST = JOINT + OFFSETS + Q_TILE, HALF_SM = 112 * 1024 + 512;
-  static constexpr int STAGES = 3 * STAGE + REST <= HALF_SM ? 3 : 2 * STAGE + REST <= HALF_SM ? 2 : 3 * STAGE + REST <= 226 * 1024 ? 3 : 2;
+  // With four row tiles a CTA computes more than it waits: three CTAs where a warp does with 168 registers (16 x 128 drafts x 8 heads of 64: 460 -> 385 us;
+  // of 128 columns, spilling, 671 -> 893)
+  static constexpr bool THIRD = MW == 4 && std::is_same<T, bf16>::value && D <= 80;
+  static constexpr int STAGES = THIRD ? 2 : 3 * STAGE + REST <= HALF_SM ? 3 : 2 * STAGE + REST <= HALF_SM ? 2 : 3 * STAGE + REST <= 226 * 1024 ? 3 : 2;
   static constexpr int SMEM = STAGES * STAGE + REST;
-  static constexpr int CTAS_PER_SM = SMEM <= HALF_SM ? 2 : 1;
+  static constexpr int CTAS_PER_SM = THIRD ? 3 : SMEM <= HALF_SM ? 2 : 1;
 };
 
 template <class T, int D, int MW>
@@ -719,7 +722,9 @@ bool rows_aligned(const ojc_tensor* t, int axes) {
 }
 
 bool tiles_take(const ojc_tensor* q, const ojc_tensor* k, const ojc_tensor* v, const ojc_tensor* out, int64_t dim) {
-  const bool shape = dim == 64 || dim == 96 || dim == 128 || (q->dtype == OJC_BF16 && (dim == 80 || dim == 256));
+  // tiles_by_dim's list
+  const bool shape = dim == 32 || dim == 48 || dim == 64 || dim == 80 || dim == 96 || dim == 112 || dim == 128 ||
+                     (q->dtype == OJC_BF16 && (dim == 160 || dim == 192 || dim == 256));
   return shape && rows_aligned(q, 2) && rows_aligned(k, 3) && rows_aligned(v, 3) && rows_aligned(out, 2);
 }
 
@@ -767,10 +772,18 @@ ojc_status tiles_by_rows(const AttnCall& c) {
 
 template <class T>
 ojc_status tiles_by_dim(const AttnCall& c) {
-  if (c.a.dim == 64) return tiles_by_rows<T, 64>(c);
-  if (c.a.dim == 96) return tiles_by_rows<T, 96>(c);
+  switch (c.a.dim) {
+    case 32: return tiles_by_rows<T, 32>(c);
+    case 48: return tiles_by_rows<T, 48>(c);
+    case 64: return tiles_by_rows<T, 64>(c);
+    case 80: return tiles_by_rows<T, 80>(c);
+    case 96: return tiles_by_rows<T, 96>(c);
+    case 112: return tiles_by_rows<T, 112>(c);
+    default: break;
+  }
   if constexpr (std::is_same<T, bf16>::value) {
-    if (c.a.dim == 80) return tiles_by_rows<T, 80>(c);
+    if (c.a.dim == 160) return tiles_by_rows<T, 160>(c);
+    if (c.a.dim == 192) return tiles_by_rows<T, 192>(c);
     if (c.a.dim == 256) return tiles_by_rows<T, 256>(c);
   }
   return tiles_by_rows<T, 128>(c);
@@ -841,6 +854,7 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
     OJC_TRY(check_tensor(op, "lse", lse));
     if (lse->dtype != OJC_F32 || lse->rank != 2 || lse->shape[0] != a.tokens || lse->shape[1] != a.heads) return ojc_fail(OJC_ERR_SHAPE, op, "lse must be F32 [N, H]");
   }
+  OJC_CUDA(be, cudaSetDevice(be->device), op);
   uint64_t need = 0;
   OJC_TRY(ojc_paged_attention_workspace_bytes(be, q, k_pages, &need));
   if (workspace) {

@@ -25,7 +25,7 @@ struct SplitUnit { int pieces, kv_head, row, rows; uint32_t first; };
 struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][tile rows][D]; ml [2 CTAs][tile rows]: maximum in log2 units, sum; split [CTAs]
 
 // Both kernels' limits: one wave of CTAs (two to an SM of the tiles kernel with 64 rows at most, one of the tcgen05 kernel with 256)
-constexpr int MAX_SHARES = 2 * REDUCE_SMS, MAX_SHARE_ROWS = REDUCE_SMS * 256;
+constexpr int MAX_SHARES = 3 * REDUCE_SMS, MAX_SHARE_ROWS = REDUCE_SMS * 256;
 
 struct AttnDims { int64_t tokens, heads, kv_heads, dim, pages, page; };
 struct AttnCall {

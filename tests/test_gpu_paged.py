@@ -602,3 +602,97 @@ def test_a_long_sequence_in_many_pieces(be, cached, h, hk, d, new, bf16):
     out, lse = c.check(be, workspace=True)
     again = c.run(be)
     assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("d", [16, 24, 32, 48, 112, 160, 192])
+def test_attention_at_other_head_dims(be, d, bf16):
+    Case(41 + d, [130, 3, 0], [9, 1, 40], 4, 2, d, 16, True, bf16).check(be)
+    Case(42 + d, [700], [1], 8, 8, d, 8, False, bf16).check(be)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("q_pad", [3, 4, 8])
+def test_attention_rows_at_any_alignment(be, bf16, q_pad):
+    Case(43, [100, 40], [9, 20], 4, 2, 64, 16, True, bf16, pad=1).check(be, q_pad=q_pad)
+
+
+@pytest.mark.parametrize("h,hk,d,page", [(4, 2, 64, 16), (2, 2, 40, 8), (8, 1, 128, 32)])
+@pytest.mark.parametrize("new", [1, 7])
+def test_attention_over_more_requests_than_a_cta_has_threads(be, h, hk, d, page, new):
+    """The lengths are scanned in chunks; requests without new tokens stand at the front, in the middle and at the end."""
+    rng = np.random.default_rng(44)
+    cached = rng.integers(0, 40, 301)
+    counts = np.where(rng.random(301) < 0.3, 0, rng.integers(1, new + 1, 301))
+    counts[[0, 1, 150, 299, 300]] = 0
+    counts[5] = new
+    Case(45, list(cached), [int(x) for x in counts], h, hk, d, page, True, True, pad=3).check(be)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("h,hk,d,new", [(4, 2, 64, [12, 3]), (8, 1, 128, [40, 33])])
+@pytest.mark.parametrize("window", [3, 40])
+@pytest.mark.parametrize("tree", [True, False])
+def test_attention_window_without_positions(be, bf16, h, hk, d, new, window, tree):
+    Case(46, [60, 0], new, h, hk, d, 16, tree, bf16).check(be, window=window, use_positions=False)
+
+
+def test_attention_leaves_rows_before_the_first_start(be):
+    for h, hk, d in ((4, 2, 64), (2, 2, 40), (16, 1, 128)):
+        c = Case(47, [90], [20], h, hk, d, 16, False, True, pad=4)
+        out, lse = c.check(be)
+        c.starts = c.starts + 3                            # the same queries three rows further on
+        c.q = np.concatenate([np.zeros((3, h, d), np.float32), c.q[:20], np.zeros((1, h, d), np.float32)])
+        c.positions = np.concatenate([np.zeros(3, np.int64), c.positions[:20], np.zeros(1, np.int64)])
+        got, got_lse = c.run(be)
+        assert np.array_equal(got[3:23], out[:20]) and np.array_equal(got_lse[3:23], lse[:20])
+        assert np.all(got[:3] == 7.0) and np.all(got[23:] == 7.0)
+
+
+def test_attention_writes_over_its_queries(be):
+    """out may be q itself: a unit's rows are written when everything that reads them has."""
+    for h, hk, d, cached, new in ((4, 2, 64, 500, 1), (8, 1, 128, 3000, 40), (2, 2, 40, 50, 4), (16, 1, 64, 2000, 5)):
+        c = Case(48, [cached, 30], [new, 2], h, hk, d, 16, True, True)
+        out, _ = c.check(be)
+        q = floats(be, c.q, True)
+        be.paged_attention_forward(q, floats(be, c.k, True), floats(be, c.v, True), u32(be, c.tables), u32(be, c.cached), u32(be, c.starts), masks=be.upload(c.masks),
+                                   positions=u32(be, c.positions), out=q)
+        assert np.array_equal(q.numpy(), out)
+
+
+def test_requests_may_share_pages_and_kv_heads_may_be_views(be):
+    """A common prefix: two requests' tables name the same pages; the pages are every other head of a wider pool."""
+    from ojas_b200 import Tensor
+    c = Case(49, [64, 64], [5, 5], 4, 2, 64, 16, True, True)
+    c.tables[1, :4] = c.tables[0, :4]
+    wide = np.zeros(c.k.shape[:2] + (4, 64), np.float32)
+    views = []
+    for pages in (c.k, c.v):
+        wide[:, :, ::2] = np.nan_to_num(pages)
+        wide[:, :, 1::2] = np.nan
+        base = floats(be, wide, True)
+        s = base.strides
+        views.append(Tensor(be, base.ptr, pages.shape, base.dtype, (s[0], s[1], 2 * s[2], 1), owner=base))
+    c.check(be, kp=views[0], vp=views[1])
+
+
+def test_pages_far_into_a_large_pool(be):
+    """Element offsets beyond 32 bits: 2.6 GB of pages a side, the request's at the very end; attention on each kernel, and the write."""
+    from ojas_b200 import DType
+    pool, page, hk, d = 41000, 64, 4, 128
+    for h, new, bf16 in ((8, 1, True), (32, 16, True)):
+        kp, vp = be.zeros((pool, page, hk, d), DType.BF16), be.zeros((pool, page, hk, d), DType.BF16)
+        c = Case(50, [200], [new], h, hk, d, page, True, bf16)
+        small = c.tables.copy()
+        c.tables = np.where(c.tables < 1000, pool - 1 - c.tables, c.tables)
+        keep_k, keep_v = c.k, c.v
+        n = 200 + new
+        at = np.arange(n)
+        slots = c.tables[0, at // page] * page + at % page
+        rows_k, rows_v = (a[small[0, at // page], at % page] for a in (keep_k, keep_v))
+        be.paged_kv_write(kp, vp, floats(be, rows_k, True), floats(be, rows_v, True), u32(be, slots))
+        got, lse = c.run(be, kp=kp, vp=vp)
+        tables, c.tables = c.tables, small
+        want, want_lse = c.run(be)
+        assert np.array_equal(got, want) and np.array_equal(lse, want_lse)
+        del kp, vp
