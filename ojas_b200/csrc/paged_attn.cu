@@ -854,12 +854,13 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
     OJC_TRY(check_tensor(op, "lse", lse));
     if (lse->dtype != OJC_F32 || lse->rank != 2 || lse->shape[0] != a.tokens || lse->shape[1] != a.heads) return ojc_fail(OJC_ERR_SHAPE, op, "lse must be F32 [N, H]");
   }
-  OJC_CUDA(be, cudaSetDevice(be->device), op);
   uint64_t need = 0;
   OJC_TRY(ojc_paged_attention_workspace_bytes(be, q, k_pages, &need));
   if (workspace) {
     if (workspace_bytes < need || ((uintptr_t)workspace & 255)) return ojc_fail(OJC_ERR_SHAPE, op, "the workspace is too small or not 256-byte aligned");
-  } else {
+  }
+  OJC_CUDA(be, cudaSetDevice(be->device), op);   // the caller's current device may be another backend's
+  if (!workspace) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     OJC_CUDA(be, cudaStreamIsCapturing(be->stream, &capturing), op);
     if (capturing != cudaStreamCaptureStatusNone) return ojc_fail(OJC_ERR_UNSUPPORTED, op, "a call that is captured into a graph needs a workspace of its own");
