@@ -752,8 +752,8 @@ ojc_status tiles_launch(const AttnCall& c) {
   cfg.numAttrs = 1;
   OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tiles_kernel<T, D, MW>, rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
                                     rows_view<T>(c.out), c.lse, c.work, (int)c.a.heads, group, (int)c.a.kv_heads, c.scale, c.be->fault_dev), c.op);
-  c.be->launches++;
-  return paged_attention_join(c, ctas, 16 * MW);
+  OJC_LAUNCHED(c.be, c.op);
+  return c.ix.width * c.ix.page <= S::KEYS ? OJC_OK : paged_attention_join(c, ctas, 16 * MW);   // no unit of one block is ever shared
 }
 
 template <class T, int D>

@@ -576,8 +576,8 @@ ojc_status launch(const AttnCall& c) {
   cfg.attrs = &early;
   cfg.numAttrs = 1;
   OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tcgen05_kernel<D, T>, mk, mv, args), c.op);
-  c.be->launches++;
-  return paged_attention_join(c, ctas, ROWS * T);
+  OJC_LAUNCHED(c.be, c.op);
+  return c.ix.width * c.ix.page <= KEYS ? OJC_OK : paged_attention_join(c, ctas, ROWS * T);   // no unit of one block is ever shared
 }
 
 }  // namespace
