@@ -583,6 +583,244 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
 }
 
+// ======================================================================== few rows in F32
+// Up to four rows to a KV head in F32, where the tiles' split products (three MMAs on 16 rows, each operand taken apart) cost more than the bytes: plain
+// fused multiply-adds. A warp takes 16 keys of a block of 64: for the scores a pair of lanes shares a key, alternating chunks of 16 bytes (rows of D + 8
+// words: no bank conflicts); for the output a lane keeps D / 32 columns and the keys' weights come by shuffles. The line of work, the copies and the joining are the
+// tiles kernel's. Bound by the cache's bytes: 12 x 64 heads over 60,000 places 65 us, 5.7 TB/s, against 113 on the
+// tiles; 8 x 4000 places of 12 x 128 51 us against 97.
+template <int D, int R> struct FewShape {
+  static constexpr int PITCH = D + 8, KEYS = 64, STAGE = 2 * KEYS * PITCH * 4, JOINT = 3 * R * (D + 2) * 4, OFFSETS = 2 * KEYS * 8, Q_TILE = R * D * 4;
+  static constexpr int REST = JOINT + OFFSETS + Q_TILE, HALF_SM = 113 * 1024;
+  static constexpr int STAGES = 3 * STAGE + REST <= HALF_SM ? 3 : 2 * STAGE + REST <= HALF_SM ? 2 : 3;
+  static constexpr int SMEM = STAGES * STAGE + REST, CTAS_PER_SM = SMEM <= HALF_SM ? 2 : 1;
+};
+
+template <int D, int R>
+__global__ void __launch_bounds__(TILE_WARPS * 32, FewShape<D, R>::CTAS_PER_SM)
+paged_attention_few_kernel(RowsView<const float> q, PagesView<const float> kp, PagesView<const float> vp, PassIndex ix, RowsView<float> out, float* __restrict__ lse, TileWork work, int heads,
+                           int group, int kv_heads, float scale, uint32_t* fault) {
+  using S = FewShape<D, R>;
+  constexpr int KEYS = S::KEYS, STAGES = S::STAGES, COLS = D / 32, CHUNKS = D / 4;
+  extern __shared__ __align__(128) uint8_t raw[];
+  uint64_t* rows_at = reinterpret_cast<uint64_t*>(raw + STAGES * S::STAGE);
+  float* q_tile = reinterpret_cast<float*>(rows_at + 2 * KEYS);
+  float* joint = q_tile + R * D;                                             // [3 R][D], then (m, l) of each
+  float* jm = joint + 3 * R * D;
+  __shared__ ShareScratch s_share;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  bool bad = false, wrong = false;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid == 0) work.split[blockIdx.x].pieces = 0;
+  Share<KEYS> share;
+  const bool any_work = find_share<KEYS, TILE_WARPS * 32>(ix, group, R, kv_heads, &s_share, &share, &bad);
+  if (bad) raise_fault(fault, OP_PAGED_RANGE);
+  if (!any_work) return;
+  const uint32_t begin = share.begin;
+  const int todo = share.todo;
+  Cursor<KEYS> use = share.at, ahead = use;
+  // copies: lane l looks up key l's row of K, lane 16 + l its row of V; places behind the last one repeat it
+  struct Place { uint32_t id, off; int hk; };
+  auto look_up = [&]() {
+    Place p;
+    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * KEYS + 16 * warp + (lane & 15)), last);
+    const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
+    p.off = j - pi * ix.page;
+    p.id = ix.tables[(int64_t)ahead.b * ix.width + pi];
+    p.hk = ahead.hk;
+    ahead.step(ix, group, R, kv_heads, &bad);
+    return p;
+  };
+  uint64_t* my_rows = rows_at + warp * 32;
+  auto copy_block = [&](int stage, Place p) {
+    if (p.id >= ix.pages) { bad = true; p.id = 0; }
+    my_rows[lane] = lane < 16 ? (uint64_t)(kp.ptr + p.id * kp.sp + p.off * kp.st + p.hk * kp.sh) : (uint64_t)(vp.ptr + p.id * vp.sp + p.off * vp.st + p.hk * vp.sh);
+    __syncwarp();
+    const uint32_t k0 = smem_addr(raw) + stage * S::STAGE + 16 * warp * S::PITCH * 4, v0 = k0 + KEYS * S::PITCH * 4;
+#pragma unroll
+    for (int i = 0; i < CHUNKS / 2; ++i) {
+      const int n = lane + 32 * i, row = n / CHUNKS, c = n % CHUNKS * 16;
+      copy16(k0 + row * S::PITCH * 4 + c, (const char*)my_rows[row] + c);
+      copy16(v0 + row * S::PITCH * 4 + c, (const char*)my_rows[16 + row] + c);
+    }
+    __syncwarp();
+  };
+  float o[R][COLS], m[R], l[R];
+  bool any[R];
+  uint32_t from[R], from_most = 0;
+  int local[R], rows = 0;
+  const float c2 = scale * LOG2_E;
+  uint32_t piece_begin = begin;
+  auto begin_unit = [&](uint32_t at) {
+    piece_begin = at;
+    from_most = 0;
+    rows = min(R, use.r.fresh * group - use.row_tile * R);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int n = use.row_tile * R + (r < rows ? r : 0);
+      local[r] = n / group;
+      from[r] = 0;
+      if (ix.window > 0) {
+        const uint32_t place = ix.positions ? ix.positions[use.r.first + local[r]] : use.r.cached + (uint32_t)local[r];
+        if (place < use.r.cached) bad = true;
+        from[r] = place >= ix.window ? place - (uint32_t)ix.window + 1 : 0;
+        from_most = max(from_most, from[r]);
+      }
+      m[r] = -INFINITY; l[r] = 0.0f; any[r] = false;
+#pragma unroll
+      for (int i = 0; i < COLS; ++i) o[r][i] = 0.0f;
+    }
+    __syncthreads();                                                          // the unit before has been computed
+    for (int i = tid; i < R * CHUNKS; i += TILE_WARPS * 32) {
+      const int r = i / CHUNKS, c = i % CHUNKS, n = use.row_tile * R + (r < rows ? r : 0);   // rows that are not there repeat the first
+      copy16(smem_addr(q_tile + r * D + 4 * c), q.ptr + (int64_t)(use.r.first + n / group) * q.sn + (int64_t)(use.hk * group + n % group) * q.sh + 4 * c);
+    }
+    if (at != begin) { copies_commit(); copies_wait<0>(); __syncthreads(); }
+  };
+  Place next_place;
+  {
+    Place p[STAGES];
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) if (i < todo) p[i] = look_up();
+    begin_unit(begin);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (i < todo) copy_block(i, p[i]);
+      copies_commit();
+    }
+    next_place = p[STAGES - 1];
+  }
+  int stage = 0;
+  for (int f = 0; f < todo; ++f) {
+    if (f > 0 && use.block == 0) begin_unit(begin + f);
+    copies_wait<STAGES - 2>();
+    if (f > 0) __syncwarp(); else __syncthreads();
+    const int next = f + STAGES - 1;
+    if (next < todo) { copy_block(stage == 0 ? STAGES - 1 : stage - 1, next_place); if (next + 1 < todo) next_place = look_up(); }
+    copies_commit();
+    const float* kt = reinterpret_cast<const float*>(raw + stage * S::STAGE) + 16 * warp * S::PITCH;
+    const float* vt = kt + KEYS * S::PITCH;
+    const uint32_t j0 = (uint32_t)((use.r.first_block + use.block) * KEYS + 16 * warp), j = j0 + (lane >> 1);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    // scores: lanes 2 k and 2 k + 1 share key k
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = 0.0f;
+    const float* krow = kt + (lane >> 1) * S::PITCH + 4 * (lane & 1);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(krow + 8 * i);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float4 y = *reinterpret_cast<const float4*>(q_tile + r * D + 8 * i + 4 * (lane & 1));
+        s[r] = fmaf(x.x, y.x, s[r]); s[r] = fmaf(x.y, y.y, s[r]); s[r] = fmaf(x.z, y.z, s[r]); s[r] = fmaf(x.w, y.w, s[r]);
+      }
+    }
+    const bool masked = j0 + 16 > use.r.cached || j0 < from_most;
+    uint32_t sees[R];                                                          // by lanes
+    float p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+      bool v = true;
+      if (masked) {
+        if (j < use.r.cached) v = j >= from[r];
+        else {
+          const uint32_t d = j - use.r.cached;
+          v = d < (uint32_t)use.r.fresh;
+          if (v) v = ix.masks ? (d >> 5) < (uint32_t)ix.words && (ix.masks[(int64_t)(use.r.first + local[r]) * ix.words + (d >> 5)] >> (d & 31) & 1u) : d <= (uint32_t)local[r];
+          if (v && ix.window > 0) v = (ix.positions ? ix.positions[use.r.first + d] : j) >= from[r];
+        }
+      }
+      sees[r] = __ballot_sync(0xffffffffu, v);
+      any[r] |= sees[r] != 0;
+      const float top = fmaxf(m[r], warp_max(v ? s[r] : -INFINITY)), base = top == -INFINITY ? 0.0f : top * c2, corr = exp2_fast(fmaf(m[r], c2, -base));
+      p[r] = v ? exp2_fast(fmaf(s[r], c2, -base)) : 0.0f;
+      l[r] = fmaf(l[r], corr, 0.5f * warp_sum(p[r]));                          // every key stands twice
+      if (top != m[r]) {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) o[r][i] *= corr;
+      }
+      m[r] = top;
+    }
+    // output: a key's weight from its lanes; places that a row does not see are left out, whatever they hold
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      float v[COLS];
+      const float* vrow = vt + k * S::PITCH + lane * COLS;
+      if constexpr (COLS == 4) { const float4 x = *reinterpret_cast<const float4*>(vrow); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+      else if constexpr (COLS == 2) { const float2 x = *reinterpret_cast<const float2*>(vrow); v[0] = x.x; v[1] = x.y; }
+      else {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) v[i] = vrow[i];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w = __shfl_sync(0xffffffffu, p[r], 2 * k);
+        if (sees[r] >> (2 * k) & 1u) {
+#pragma unroll
+          for (int i = 0; i < COLS; ++i) o[r][i] = fmaf(w, v[i], o[r][i]);
+        }
+      }
+    }
+    const bool unit_done = use.block + 1 == use.r.blocks;
+    if (unit_done || f + 1 == todo) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) if (any[r] && m[r] == -INFINITY) l[r] = NAN;     // every score -inf: what the formula gives
+      __syncthreads();                                                          // what a unit before left has been taken
+      if (warp > 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int at = (warp - 1) * R + r;
+#pragma unroll
+          for (int i = 0; i < COLS; ++i) joint[at * D + lane * COLS + i] = o[r][i];
+          if (lane == 0) { jm[2 * at] = m[r]; jm[2 * at + 1] = l[r]; }
+        }
+      }
+      __syncthreads();
+      const uint32_t unit_begin = begin + f - use.block;
+      const bool starts = piece_begin == unit_begin, whole = unit_done && starts;
+      if (warp == 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (r >= rows) continue;
+#pragma unroll
+          for (int w = 0; w < TILE_WARPS - 1; ++w) {
+            const int at = w * R + r;
+            const float m2 = jm[2 * at], l2 = jm[2 * at + 1], top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.0f : top * c2;
+            const float ca = exp2_fast(fmaf(m[r], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
+            l[r] = l[r] * ca + l2 * cb;
+            m[r] = top;
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) o[r][i] = o[r][i] * ca + joint[at * D + lane * COLS + i] * cb;
+          }
+          const int n = use.row_tile * R + r, h = use.hk * group + n % group;
+          const int64_t t = use.r.first + local[r];
+          if (whole) {
+            const bool seen = !(m[r] == -INFINITY && l[r] == 0.0f);
+            const float inv = seen ? 1.0f / l[r] : 0.0f;
+            float* po = out.ptr + t * out.sn + h * out.sh + lane * COLS;
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) { const float x = o[r][i] * inv; wrong |= !isfinite(x); po[i] = x; }
+            if (lane == 0 && lse) lse[t * heads + h] = seen ? m[r] * scale + logf(l[r]) : -INFINITY;
+          } else {
+            const int64_t row = (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * R + r;
+            if (lane == 0) work.ml[row] = make_float2(m[r] * c2, l[r]);
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) work.o[row * D + lane * COLS + i] = o[r][i];
+          }
+        }
+      }
+      if (!unit_done && starts && tid == 0)
+        work.split[blockIdx.x] = SplitUnit{(int)(share.of_block(unit_begin + use.r.blocks - 1) - blockIdx.x) + 1, use.hk, use.row_tile * R, rows, use.r.first};
+    }
+    use.step(ix, group, R, kv_heads, &bad);
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (bad) raise_fault(fault, OP_PAGED_RANGE);
+  else if (wrong) raise_fault(fault, OP_PAGED_ATTN);
+}
+
 // Joins the pieces of the units that several CTAs shared: blocks (c, .) take the unit whose first piece CTA c left. A warp takes a row, or where a unit has
 // many pieces a 2nd, 4th or 8th part of a row's (joined in a fixed order); lanes are columns. The loads of four pieces, maxima and outputs, are in
 // flight together: two round trips to memory for a unit of up to four pieces (latency is all there is to this kernel, so registers are kept few: with
@@ -728,16 +966,15 @@ bool tiles_take(const ojc_tensor* q, const ojc_tensor* k, const ojc_tensor* v, c
   return shape && rows_aligned(q, 2) && rows_aligned(k, 3) && rows_aligned(v, 3) && rows_aligned(out, 2);
 }
 
-template <class T, int D, int MW>
-ojc_status tiles_launch(const AttnCall& c) {
-  using S = TileShape<T, D, MW>;
-  static PerDeviceFlag attr;
+// Launches a kernel with the shape S on tiles of `tile_rows` rows, and the join behind it.
+template <class T, class S, class Kernel>
+ojc_status shares_launch(const AttnCall& c, Kernel kernel, int tile_rows) {
+  static PerDeviceFlag attr;                                                 // one for each S, and so for each kernel
   if (!attr[c.be->device]) {
-    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tiles_kernel<T, D, MW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), c.op);
+    OJC_CUDA(c.be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), c.op);
     attr[c.be->device] = true;
   }
-  static_assert(S::CTAS_PER_SM * REDUCE_SMS <= MAX_SHARES && S::CTAS_PER_SM * REDUCE_SMS * 16 * MW <= MAX_SHARE_ROWS, "workspace");
-  const unsigned ctas = attn_ctas(c, S::CTAS_PER_SM * REDUCE_SMS, 16 * MW, S::KEYS);
+  const unsigned ctas = attn_ctas(c, S::CTAS_PER_SM * REDUCE_SMS, tile_rows, S::KEYS);
   const int group = (int)(c.a.heads / c.a.kv_heads);
   // queued while the kernel before still runs; it waits for that one's end before it looks at memory
   cudaLaunchAttribute early;
@@ -750,11 +987,21 @@ ojc_status tiles_launch(const AttnCall& c) {
   cfg.stream = c.be->stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tiles_kernel<T, D, MW>, rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix,
-                                    rows_view<T>(c.out), c.lse, c.work, (int)c.a.heads, group, (int)c.a.kv_heads, c.scale, c.be->fault_dev), c.op);
+  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, kernel, rows_view<const T>(c.q), pages_view<const T>(c.k), pages_view<const T>(c.v), c.ix, rows_view<T>(c.out), c.lse, c.work, (int)c.a.heads, group,
+                                    (int)c.a.kv_heads, c.scale, c.be->fault_dev), c.op);
   OJC_LAUNCHED(c.be, c.op);
-  return c.ix.width * c.ix.page <= S::KEYS ? OJC_OK : paged_attention_join(c, ctas, 16 * MW);   // no unit of one block is ever shared
+  return c.ix.width * c.ix.page <= S::KEYS ? OJC_OK : paged_attention_join(c, ctas, tile_rows);   // no unit of one block is ever shared
 }
+
+template <class T, int D, int MW>
+ojc_status tiles_launch(const AttnCall& c) {
+  using S = TileShape<T, D, MW>;
+  static_assert(S::CTAS_PER_SM * REDUCE_SMS <= MAX_SHARES && S::CTAS_PER_SM * REDUCE_SMS * 16 * MW <= MAX_SHARE_ROWS, "workspace");
+  return shares_launch<T, S>(c, paged_attention_tiles_kernel<T, D, MW>, 16 * MW);
+}
+
+template <int D, int R>
+ojc_status few_launch(const AttnCall& c) { return shares_launch<float, FewShape<D, R>>(c, paged_attention_few_kernel<D, R>, R); }
 
 template <class T, int D>
 ojc_status tiles_by_rows(const AttnCall& c) {
@@ -765,6 +1012,11 @@ ojc_status tiles_by_rows(const AttnCall& c) {
   // page copies by boxes count (20 rows over 131 thousand: 107 against 123 us).
   const bool wide = rows > 32 || (rows > 16 && c.ix.width * c.ix.page >= 32768);
   if ((D == 64 || D == 128) && wide && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
+  if constexpr (std::is_same<T, float>::value && D % 32 == 0) {
+    if (rows == 1) return few_launch<D, 1>(c);
+    if (rows == 2) return few_launch<D, 2>(c);
+    if (rows <= 4) return few_launch<D, 4>(c);
+  }
   if (rows <= 16) return tiles_launch<T, D, 1>(c);
   if (rows <= 32) return tiles_launch<T, D, 2>(c);
   return tiles_launch<T, D, 4>(c);
@@ -796,7 +1048,7 @@ ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_row
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(shares, tile_rows / (tile_rows <= 64 ? 4 : 8));   // rows go round: any grid does, these leave a warp one row of most units
+  cfg.gridDim = dim3(shares, std::max(1, tile_rows / (tile_rows <= 64 ? 4 : 8)));   // rows go round: any grid does, these leave a warp one row of most units
   cfg.blockDim = dim3(JOIN_WARPS * 32);
   cfg.dynamicSmemBytes = JOIN_WARPS * c.a.dim * 4;
   cfg.stream = c.be->stream;
