@@ -108,7 +108,7 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 // ======================================================================== tiles on the tensor cores
 // Row tiles of 16 * MW rows, key blocks of 64 or 128 (paged_attn.cuh has the line of work).
 //
-// What bounds it: the cache's bytes for few rows. Four warps to a CTA, two CTAs to an SM, three stages of 64 keys each, rows fetched by 16-byte asynchronous
+// What bounds it: the cache's bytes for few rows. Four warps to a CTA, one to three CTAs to an SM, two or three stages of 64 or 128 keys each, rows fetched by 16-byte asynchronous
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
 // Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
@@ -1010,8 +1010,10 @@ ojc_status tiles_by_rows(const AttnCall& c) {
   // More than 32 rows: tcgen05 (48 drafts over 4000 cached, 16 heads of 128: 55 us against 76; 100 drafts 61 against 117). 17 to 32 rows: its tiles of 128 rows
   // are mostly empty and the tiles here are ahead (31 drafts: 51 against 57 us at 1000 cached, 60 against 62 at 4000), except over long contexts, where the
   // page copies by boxes count (20 rows over 131 thousand: 107 against 123 us).
-  const bool wide = rows > 32 || (rows > 16 && c.ix.width * c.ix.page >= 32768);
-  if ((D == 64 || D == 128) && wide && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
+  // Heads that leave columns of the operands empty, 63 rows: 68 us here against 63 at 96 columns and 4000 cached, 77 against 83 at 300 cached, 43 against 56 at
+  // 32 columns; from 65 rows on a unit here is two row tiles (255 rows: 573 us against 208 at 96 columns, 282 against 180 at 32).
+  const bool whole = D == 64 || D == 128, wide = whole ? rows > 32 || (rows > 16 && c.ix.width * c.ix.page >= 32768) : rows > 64;
+  if (D <= 128 && wide && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
   if constexpr (std::is_same<T, float>::value && D % 32 == 0) {
     if (rows == 1) return few_launch<D, 1>(c);
     if (rows == 2) return few_launch<D, 2>(c);

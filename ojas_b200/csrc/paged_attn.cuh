@@ -24,7 +24,7 @@ struct PassIndex {       // the pass's index tables (all U32)
 struct SplitUnit { int pieces, kv_head, row, rows; uint32_t first; };
 struct TileWork { float* o; float2* ml; SplitUnit* split; };   // o [2 CTAs][tile rows][D]; ml [2 CTAs][tile rows]: maximum in log2 units, sum; split [CTAs]
 
-// Both kernels' limits: one wave of CTAs (two to an SM of the tiles kernel with 64 rows at most, one of the tcgen05 kernel with 256)
+// Both kernels' limits: one wave of CTAs (up to three to an SM of the tiles kernel with 64 rows at most, one of the tcgen05 kernel with 256)
 constexpr int MAX_SHARES = 3 * REDUCE_SMS, MAX_SHARE_ROWS = REDUCE_SMS * 256;
 
 struct AttnDims { int64_t tokens, heads, kv_heads, dim, pages, page; };
@@ -41,7 +41,7 @@ inline unsigned attn_ctas(const AttnCall& c, int wave, int tile_rows, int keys) 
 }
 // The joining kernel behind one that ran `shares` CTAs with tiles of `tile_rows` rows
 ojc_status paged_attention_join(const AttnCall& c, unsigned shares, int tile_rows);
-// tcgen05 / TMEM form with one or two tiles of 128 rows (BF16, head_dim 64 or 128, pages that tile 128 keys)
+// tcgen05 / TMEM form with one or two tiles of 128 rows (BF16, head dims up to 128 of the tiles kernel, pages that tile 128 keys)
 bool paged_attention_tcgen05_takes(const AttnCall& c);
 ojc_status paged_attention_tcgen05(const AttnCall& c, int tiles);
 

@@ -1,5 +1,6 @@
 // Paged attention for many rows to a KV head on the Blackwell tensor cores (tcgen05 + TMEM): trees of drafts times the query heads of a group, and
-// pieces of prompts. BF16, head_dim 64 or 128.
+// pieces of prompts. BF16, head dims of the tiles up to 128: the operands have D = 64 or 128 columns, those behind the head's are zeros (TMA fills them
+// in for K and V).
 //
 // A CTA walks its stretch of the line of work (paged_attn.cuh) in blocks of 128 keys with T = 1 or 2 tiles of 128 rows:
 //   warps 0 .. 4T-1  softmax, one thread per row (= TMEM lane): at a unit's start the row of Q into shared memory (swizzled K-major operand) and zeros
@@ -59,7 +60,7 @@ struct TcArgs {
   float* lse;
   PassIndex ix;
   TileWork work;
-  int heads, group, kv_heads;
+  int heads, group, kv_heads, dim;
   int k_heads_inside, v_heads_inside;   // tensor-map order: (D, Hkv, page, P) or (D, page, Hkv, P)
   int out_sectors;                      // out's rows start at 32-byte boundaries
   int box_rows;                         // rows of a page that one box holds: min(page, 128)
@@ -103,8 +104,8 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
 
 // A warp's 32 rows of a Q tile, asynchronously into the swizzled operand at `tile` (row pointers from the lanes that own the rows). Not inlined: it runs once
 // to a unit, and its addresses would cost the softmax loop its registers.
-template <int D>
-__device__ __noinline__ void fetch_q_rows(RowsView<const bf16> q, uint32_t first, int fresh, int hk, int row0, int group, uint32_t tile) {
+template <int D, bool WHOLE>
+__device__ __noinline__ void fetch_q_rows(RowsView<const bf16> q, uint32_t first, int fresh, int hk, int row0, int group, int dim, uint32_t tile) {
   const int lane = threadIdx.x & 31, t0 = threadIdx.x & 96, n = row0 + t0 + lane;
   const uint64_t mine = n < fresh * group ? (uint64_t)(q.ptr + (int64_t)(first + (uint32_t)(n / group)) * q.sn + (int64_t)(hk * group + n % group) * q.sh) : 0;
   const int c = lane % (D / 8);
@@ -113,14 +114,18 @@ __device__ __noinline__ void fetch_q_rows(RowsView<const bf16> q, uint32_t first
   for (int i = 0; i < D / 8; ++i) {
     const int row = i * (256 / D) + lane / (D / 8);
     const uint64_t from = __shfl_sync(0xffffffffu, mine, row);
-    if (from) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(from + c * 16) : "memory");
+    const uint32_t to = dst + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+    if (!WHOLE && 8 * c >= dim) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+    else if (from) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + c * 16) : "memory");
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-template <int D, int T>
+// WHOLE: the head has all D columns (asked at run time, a tree of 63 drafts took 2 % longer, most of it in the fetching of Q)
+template <int D, int T, bool WHOLE>
 __global__ void __launch_bounds__(Shape<D, T>::THREADS, 1)
 paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcArgs args) {
+  const int dim = WHOLE ? D : args.dim;
   using C = Shape<D, T>;
   constexpr int STAGES = C::STAGES, TILE_ROWS = ROWS * T;
   constexpr uint32_t TILE16 = C::TILE_BYTES >> 4;
@@ -302,7 +307,7 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
     };
     // The Q tile of a unit: a warp fetches its 32 rows together (row pointers from the lanes that own them), asynchronously, straight into the swizzled
     // operand. It is called as soon as the last S of the unit before is there, so the copies run under that unit's last softmax.
-    auto fetch_q = [&](const Cursor<KEYS>& u) { fetch_q_rows<D>(args.q, u.r.first, u.r.fresh, u.hk, u.row_tile * TILE_ROWS + g * ROWS, args.group, base + g * C::TILE_BYTES); };
+    auto fetch_q = [&](const Cursor<KEYS>& u) { fetch_q_rows<D, WHOLE>(args.q, u.r.first, u.r.fresh, u.hk, u.row_tile * TILE_ROWS + g * ROWS, args.group, dim, base + g * C::TILE_BYTES); };
     auto give_q = [&]() {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       fence_async_smem();
@@ -494,6 +499,7 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
             if (row.live && whole) {
 #pragma unroll
               for (int i = 0; i < 32; i += 16) {
+                if (!WHOLE && c * 32 + i >= dim) break;
                 uint32_t w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -507,8 +513,9 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
             } else if (row.live) {
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
+                if (!WHOLE && c * 32 + i >= dim) break;
                 const uint32_t w[8] = {o[i], o[i + 1], o[i + 2], o[i + 3], o[i + 4], o[i + 5], o[i + 6], o[i + 7]};
-                store32(args.work.o + at * D + c * 32 + i, w);
+                store32(args.work.o + at * dim + c * 32 + i, w);
               }
             }
           }
@@ -549,15 +556,19 @@ ojc_status pages_map(const AttnCall& c, CUtensorMap* map, const ojc_tensor* t, b
   return OJC_OK;
 }
 
-template <int D, int T>
+template <int D, int T, bool WHOLE>
 ojc_status launch(const AttnCall& c) {
   using S = Shape<D, T>;
   static PerDeviceFlag attr;
   if (!attr[c.be->device]) {
-    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tcgen05_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), c.op);
+    // the register shares of T 2 add up to 168 for each of the launched threads: with fewer their second half would wait for ever
+    cudaFuncAttributes made;
+    OJC_CUDA(c.be, cudaFuncGetAttributes(&made, paged_attention_tcgen05_kernel<D, T, WHOLE>), c.op);
+    if (T == 2 && made.numRegs < 168) return ojc_fail(OJC_ERR_BACKEND, c.op, "the kernel was built with fewer registers than its warps share out");
+    OJC_CUDA(c.be, cudaFuncSetAttribute(paged_attention_tcgen05_kernel<D, T, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), c.op);
     attr[c.be->device] = true;
   }
-  TcArgs args{rows_view<const bf16>(c.q), rows_view<bf16>(c.out), c.lse, c.ix, c.work, (int)c.a.heads, (int)(c.a.heads / c.a.kv_heads), (int)c.a.kv_heads,
+  TcArgs args{rows_view<const bf16>(c.q), rows_view<bf16>(c.out), c.lse, c.ix, c.work, (int)c.a.heads, (int)(c.a.heads / c.a.kv_heads), (int)c.a.kv_heads, (int)c.a.dim,
               c.k->stride[2] < c.k->stride[1], c.v->stride[2] < c.v->stride[1],
               (uintptr_t)c.out->data % 32 == 0 && c.out->stride[0] % 16 == 0 && c.out->stride[1] % 16 == 0, (int)std::min<int64_t>(c.a.page, KEYS), c.scale, c.be->fault_dev};
   CUtensorMap mk, mv;
@@ -575,7 +586,7 @@ ojc_status launch(const AttnCall& c) {
   cfg.stream = c.be->stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tcgen05_kernel<D, T>, mk, mv, args), c.op);
+  OJC_CUDA(c.be, cudaLaunchKernelEx(&cfg, paged_attention_tcgen05_kernel<D, T, WHOLE>, mk, mv, args), c.op);
   OJC_LAUNCHED(c.be, c.op);
   return c.ix.width * c.ix.page <= KEYS ? OJC_OK : paged_attention_join(c, ctas, ROWS * T);   // no unit of one block is ever shared
 }
@@ -583,7 +594,7 @@ ojc_status launch(const AttnCall& c) {
 }  // namespace
 
 bool paged_attention_tcgen05_takes(const AttnCall& c) {
-  if (!c.be->tmap_encode || c.q->dtype != OJC_BF16 || (c.a.dim != 64 && c.a.dim != 128)) return false;
+  if (!c.be->tmap_encode || c.q->dtype != OJC_BF16 || c.a.dim > 128 || c.a.dim % 16) return false;
   if (c.a.page % 8 || (KEYS % c.a.page && c.a.page % KEYS)) return false;    // boxes of whole 8-row swizzle groups that tile a block
   for (const ojc_tensor* t : {c.k, c.v})
     for (int i = 0; i < 3; ++i) if (t->stride[i] <= 0 || t->stride[i] >= 1ll << 38) return false;   // what a tensor map can say
@@ -591,6 +602,8 @@ bool paged_attention_tcgen05_takes(const AttnCall& c) {
 }
 
 ojc_status paged_attention_tcgen05(const AttnCall& c, int tiles) {
-  if (c.a.dim == 64) return tiles == 1 ? launch<64, 1>(c) : launch<64, 2>(c);
-  return tiles == 1 ? launch<128, 1>(c) : launch<128, 2>(c);
+  if (c.a.dim == 64) return tiles == 1 ? launch<64, 1, true>(c) : launch<64, 2, true>(c);
+  if (c.a.dim == 128) return tiles == 1 ? launch<128, 1, true>(c) : launch<128, 2, true>(c);
+  if (c.a.dim < 64) return tiles == 1 ? launch<64, 1, false>(c) : launch<64, 2, false>(c);
+  return tiles == 1 ? launch<128, 1, false>(c) : launch<128, 2, false>(c);
 }

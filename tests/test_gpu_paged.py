@@ -696,3 +696,74 @@ def test_pages_far_into_a_large_pool(be):
         want, want_lse = c.run(be)
         assert np.array_equal(got, want) and np.array_equal(lse, want_lse)
         del kp, vp
+
+
+@pytest.mark.parametrize("d", [16, 32, 48, 80, 96, 112])
+@pytest.mark.parametrize("new", [[20, 35], [40, 35], [200, 131]])
+def test_many_rows_at_head_dims_below_the_operands(be, d, new):
+    """tcgen05 operands of 64 and 128 columns with zeros behind the head's: values next to the head in memory (another head's) stay out."""
+    c = Case(51 + d, [700, 90], new, 2, 1, d, 16, True, True, pad=1)
+    out, lse = c.check(be)
+    again = c.check(be, heads_first=True, workspace=True)
+    assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+    c.masks[:, 0] &= np.uint32(0xFFFFFFF5)                  # a poisoned draft that no row sees
+    p, off = c.slot(1, 90 + 1)
+    c.k[p, off], c.v[p, off] = np.nan, np.inf
+    c.check(be)
+
+
+FEW = [([700, 90, 0], [1, 1, 1]), ([300, 64], [2, 3]), ([130, 1], [4, 4])]
+
+
+@pytest.mark.parametrize("cached,new", FEW)
+@pytest.mark.parametrize("h,hk", [(2, 2), (4, 2)])
+@pytest.mark.parametrize("d,page", [(32, 16), (64, 5), (96, 64), (128, 24)])
+@pytest.mark.parametrize("window", [None, 1, 70])
+@pytest.mark.parametrize("tree", [True, False])
+def test_few_rows_in_f32(be, cached, new, h, hk, d, page, window, tree):
+    """One, two and four rows to a KV head (and the eight beyond them), requests with more rows than the average among them."""
+    c = Case(60 + d, cached, new, h, hk, d, page, tree, False, words_more=1, pad=1)
+    out, lse = c.check(be, window=window)
+    again = c.run(be, window=window, workspace=True, heads_first=True)
+    assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+    c.check(be, window=window, use_positions=False)
+
+
+@pytest.mark.parametrize("h,hk,new", [(2, 2, [4, 1]), (4, 2, [2, 2]), (4, 1, [1, 1]), (3, 3, [4, 4])])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_few_rows_in_f32_that_see_nothing_and_places_that_hold_anything(be, h, hk, new, d):
+    c = Case(61 + d, [0, 100], new, h, hk, d, 16, True, False)
+    c.masks[:] &= np.uint32(0xFFFFFFFD)                    # draft 1 of each request drops out of every row
+    c.masks[0] = 0                                         # request 0 has no cache: its row 0 sees nothing
+    for b in range(2):
+        if new[b] > 1:
+            p, off = c.slot(b, int(c.cached[b]) + 1)
+            c.k[p, off], c.v[p, off] = np.nan, np.inf
+    out, lse = c.check(be)
+    assert not out[0].any() and np.all(np.isneginf(lse[0]))
+
+
+@pytest.mark.parametrize("requests,cached,h,hk,d,new", [(40, 900, 6, 6, 64, 1), (9, 3000, 2, 2, 128, 2), (150, 61, 3, 1, 96, 1)])
+def test_few_rows_in_f32_with_several_units_to_a_share(be, requests, cached, h, hk, d, new):
+    rng = np.random.default_rng(62)
+    c = Case(62, [int(x) for x in rng.integers(0, cached, requests)], [int(x) for x in rng.integers(0, new + 1, requests - 1)] + [new], h, hk, d, 16, True, False)
+    out, lse = c.check(be)
+    for _ in range(3):
+        again = c.run(be)
+        assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+
+
+def test_few_rows_in_f32_with_infinite_scores(be):
+    """Every score of a row -inf is NaN in the formula, in one piece and in many; it is reported."""
+    from ojas_b200 import OjasError
+    for cached in (40, 30000):
+        c = Case(63, [cached], [1], 2, 2, 64, 16, False, False)
+        q, k = c.q.copy(), c.k.copy()
+        q[:, 0, 0], k[..., 0, 0] = -1.0, np.inf
+        out, lse = be.paged_attention_forward(floats(be, q, False), floats(be, k, False), floats(be, c.v, False), u32(be, c.tables), u32(be, c.cached), u32(be, c.starts),
+                                              lse=be.zeros(c.q.shape[:2]))
+        with pytest.raises(OjasError) as e:
+            be.sync()
+        assert e.value.kind == "NonFinite"
+        got = out.numpy()
+        assert np.all(np.isnan(got[:, 0])) and np.all(np.isfinite(got[:, 1]))
