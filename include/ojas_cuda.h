@@ -202,7 +202,7 @@ ojc_status ojc_cached_attention_forward(ojc_backend* be, const ojc_tensor* q, co
  *      depend on capacities alone, so a pass may be captured from ojc_stream into a graph (replay it on that stream; give paged_attention_forward a
  *      workspace of the caller's). All index tensors are U32; OJC_NONE stands for "no slot" and "no parent". What the host cannot see is checked on
  *      the device: a page, slot, length, position or parent out of range is never followed and surfaces as OutOfRange at the next sync (the outputs of
- *      its request are then unspecified, the other requests' are right). */
+ *      its request are then unspecified, the other requests' are right). What is written through strides has places of its own: no broadcast views. */
 #define OJC_NONE 0xffffffffu
 /* Block tables and slot maps from lengths. cached_lens, new_lens [B]; parents [N] (optional): draft i's parent as its index among the request's
  * own drafts, below i, or OJC_NONE for a child of the last cached token; without parents each token follows the one before it. New pages are taken from

@@ -63,7 +63,11 @@ class Tensor:
         self.strides = tuple(strides) if strides is not None else _contig_strides(self.shape)
         self._owner = owner  # keeps the storage alive for views
         self._owns = owner is None
-        self._ref = None     # the descriptor as the C ABI takes it, made at the first call
+        self._ref = None     # the descriptor as the C ABI takes it, made at the first call after an attribute was set
+
+    def __setattr__(self, name, value):
+        self.__dict__[name] = value
+        self.__dict__["_ref"] = None
 
     def __del__(self):
         if getattr(self, "_owns", False) and self.ptr and self.backend is not None and self.backend._handle:
@@ -102,7 +106,7 @@ def _p(t: "Tensor | None"):
     if t is None:
         return None
     if t._ref is None:
-        t._ref = C.byref(t.c())
+        t.__dict__["_ref"] = C.byref(t.c())
     return t._ref
 
 

@@ -379,6 +379,7 @@ ojc_status rope_run(ojc_backend* be, const char* op, const ojc_rope* rope, const
   OJC_TRY(check_tensor(op, "x", x, false)); OJC_TRY(check_tensor(op, "y", y, false)); OJC_TRY(check_tensor(op, "positions", positions));
   if ((x->rank != 3 && x->rank != 4) || !same_shape(x, y)) return ojc_fail(OJC_ERR_SHAPE, op, "x, y [N, H, D] or [B, T, H, D]");
   if (x->dtype != y->dtype || !is_float(x)) return ojc_fail(OJC_ERR_DTYPE, op, "x, y share F32 or BF16");
+  OJC_TRY(own_places(op, "y", y));
   if (positions->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, "positions are U32");
   if (numel(x) == 0) return ojc_fail(OJC_ERR_SHAPE, op, "empty tensor");
   const int r = x->rank;
@@ -522,6 +523,7 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
   if (k->rank != 3 || !same_shape(k, v) || k->shape[1] != k_pages->shape[2] || k->shape[2] != k_pages->shape[3]) return ojc_fail(OJC_ERR_SHAPE, op, "k, v [N, Hkv, D]");
   if (k_pages->dtype != v_pages->dtype || k->dtype != v->dtype || !is_float(k_pages) || !is_float(k)) return ojc_fail(OJC_ERR_DTYPE, op, "k and v, and the pages, share F32 or BF16");
   if (numel(k) == 0 || numel(k_pages) == 0) return ojc_fail(OJC_ERR_SHAPE, op, "empty tensor");
+  OJC_TRY(own_places(op, "k_pages", k_pages)); OJC_TRY(own_places(op, "v_pages", v_pages));
   if (k->stride[2] != 1 || v->stride[2] != 1 || k_pages->stride[3] != 1 || v_pages->stride[3] != 1) return ojc_fail(OJC_ERR_SHAPE, op, "the head_dim axis must be contiguous");
   const int64_t tokens = k->shape[0], heads = k->shape[1], dim = k->shape[2], page = k_pages->shape[1], pages = k_pages->shape[0];
   if (page > (1 << 24) || heads > INT32_MAX || dim > INT32_MAX || pages > (int64_t)OJC_NONE / page) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "slot numbers do not fit U32");

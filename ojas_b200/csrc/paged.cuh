@@ -20,6 +20,13 @@ struct RowsView {
 template <class P>
 inline RowsView<P> rows_view(const ojc_tensor* t) { return RowsView<P>{(P*)t->data, t->stride[0], t->stride[1]}; }
 
+// A tensor that is written through its strides: no axis may lie on itself (a broadcast one, of stride 0, would take the writes of all its entries)
+inline ojc_status own_places(const char* op, const char* what, const ojc_tensor* t) {
+  for (int i = 0; i < t->rank; ++i)
+    if (t->shape[i] > 1 && t->stride[i] == 0) return ojc_fail(OJC_ERR_SHAPE, op, std::string(what) + " is written and cannot be a broadcast view");
+  return OJC_OK;
+}
+
 #ifdef __CUDACC__
 // Rotation of a pair: the angle is position x frequency with the frequency in 2^-64 turns, so the product modulo 2^64 IS the angle's fraction of a
 // turn, exact to position x 2^-64 however far the position; its upper half as a signed integer is the angle / pi in [-1, 1) x 2^31. What is rounded to

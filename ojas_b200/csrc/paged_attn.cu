@@ -1090,6 +1090,7 @@ ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, con
   if (!same_shape(k_pages, v_pages) || !same_shape(q, out)) return ojc_fail(OJC_ERR_SHAPE, op, "q, out [N, H, D]; k_pages, v_pages [P, page, Hkv, D]");
   if (v_pages->dtype != q->dtype || out->dtype != q->dtype) return ojc_fail(OJC_ERR_DTYPE, op, "q, out and the pages share F32 or BF16");
   if (q->stride[2] != 1 || out->stride[2] != 1 || k_pages->stride[3] != 1 || v_pages->stride[3] != 1) return ojc_fail(OJC_ERR_SHAPE, op, "the head_dim axis must be contiguous");
+  OJC_TRY(own_places(op, "out", out));
   OJC_TRY(u32_table(op, "block_tables", block_tables, 2)); OJC_TRY(u32_table(op, "cached_lens", cached_lens, 1)); OJC_TRY(u32_table(op, "starts", starts, 1));
   const int64_t batch = cached_lens->shape[0], width = block_tables->shape[1];
   if (batch == 0 || width == 0) return ojc_fail(OJC_ERR_SHAPE, op, "every dimension must be non-zero");

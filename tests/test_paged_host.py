@@ -164,3 +164,22 @@ def test_python_plan_wants_a_capacity():
     with pytest.raises(OjasError) as e:
         be.paged_plan(t((3,), DType.U32), t((3,), DType.U32), t((9,), DType.U32), t((1,), DType.U32), t((3, 4), DType.U32), 16)
     assert e.value.kind == "Shape"
+
+
+def test_what_is_written_cannot_be_a_broadcast_view(handle):
+    u32, b16, rope = DType.U32, DType.BF16, CudaBackend.rope_plan(RopeSpec(64))
+    x, flat = t((5, 2, 64)), t((5, 2, 64), strides=(64, 0, 1))
+    assert kind(lib.ojc_rope_forward(handle, C.byref(rope), _p(x), _p(t((5,), u32)), _p(flat))) == "Shape" and "broadcast" in lib.ojc_last_error().decode()
+    pages, flat = t((8, 16, 2, 64)), t((8, 16, 2, 64), strides=(1024, 64, 0, 1))
+    for kp, vp in ((flat, pages), (pages, flat)):
+        assert kind(lib.ojc_paged_kv_write(handle, _p(kp), _p(vp), _p(x), _p(x), _p(t((5,), u32)), None, None)) == "Shape" and "broadcast" in lib.ojc_last_error().decode()
+    got = lib.ojc_paged_attention_forward(handle, _p(t((6, 4, 64), b16)), _p(t((8, 16, 2, 64), b16)), _p(t((8, 16, 2, 64), b16)), _p(t((3, 4), u32)), _p(t((3,), u32)), _p(t((4,), u32)),
+                                          None, None, C.c_int64(-1), _p(t((6, 4, 64), b16, strides=(0, 64, 1))), None, C.c_void_p(256), C.c_uint64(1 << 40))
+    assert kind(got) == "Shape" and "broadcast" in lib.ojc_last_error().decode()
+
+
+def test_a_changed_tensor_is_passed_as_it_is_now():
+    x = t((5, 2, 64))
+    assert _p(x)._obj.data == 256 and _p(x) is _p(x)
+    x.ptr, x.shape, x.strides = 512, (5, 2, 32), (128, 64, 1)
+    assert _p(x)._obj.data == 512 and list(_p(x)._obj.shape[:3]) == [5, 2, 32] and list(_p(x)._obj.stride[:3]) == [128, 64, 1]
