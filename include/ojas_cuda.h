@@ -238,7 +238,8 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
  * only those whose position is above its own minus window (the position of a cached place is the place, that of a new token its entry of positions
  * [N], at least the cached length; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). Masked places are never
  * looked at: NaN or infinity there does no harm. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
- * non-finite value that a row does see surfaces as NonFinite. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
+ * non-finite value that a row does see surfaces as NonFinite. A call with 2^31 - 1 blocks of 64 or 128 keys or more, over all row tiles and KV heads,
+ * computes nothing and surfaces as OutOfRange. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
  * NULL for the library's own (refused while the stream is being captured). */
 ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, uint64_t* bytes);
 ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, const ojc_tensor* v_pages, const ojc_tensor* block_tables, const ojc_tensor* cached_lens,

@@ -96,25 +96,26 @@ struct Share {
 struct ShareScratch { uint32_t sum[32], at; int b; Request r; };
 
 // Called by all THREADS threads of the CTA; false: nothing for it to do. Lengths are read once for up to THREADS requests, twice beyond.
+// All sums stop at MAX_LINE, where two of them still add up in 32 bits; a line that long is reported and nobody works on it: the cursor walks every
+// request, so no part of a line may be left out of its numbering (units would be taken for ones with pieces beyond the last CTA's).
+constexpr uint32_t MAX_LINE = 0x7fffffffu;
 template <int KEYS, int THREADS>
 __device__ __forceinline__ bool find_share(const PassIndex& ix, int group, int tile_rows, int kv_heads, ShareScratch* sh, Share<KEYS>* out, bool* bad) {
   constexpr int WARPS = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto blocks_of = [&](const Request& r) {
-    const unsigned long long n = (unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads);
-    *bad |= n >= 1ull << 31;
-    return n >= 1ull << 31 ? 0u : (uint32_t)n;
+    return (uint32_t)min((unsigned long long)r.blocks * (unsigned)(r.row_tiles * kv_heads), (unsigned long long)MAX_LINE);
   };
   auto scan = [&](uint32_t n, uint32_t* upto) {                  // of a chunk of requests; the chunk's sum comes back
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const uint32_t a = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += a; }
+    for (int o = 1; o < 32; o <<= 1) { const uint32_t a = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n = min(n + a, MAX_LINE); }
     __syncthreads();
     if (lane == 31) sh->sum[warp] = n;
     __syncthreads();
     *upto = n;
     uint32_t sum = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) { if (w < warp) *upto += sh->sum[w]; sum += sh->sum[w]; }
+    for (int w = 0; w < WARPS; ++w) { if (w < warp) *upto = min(*upto + sh->sum[w], MAX_LINE); sum = min(sum + sh->sum[w], MAX_LINE); }
     return sum;
   };
   Request mine = {};
@@ -124,8 +125,9 @@ __device__ __forceinline__ bool find_share(const PassIndex& ix, int group, int t
     n = 0;
     if (b0 + tid < ix.batch) { mine = load_request<KEYS>(ix, b0 + tid, group, tile_rows, bad); n = blocks_of(mine); }
     const uint32_t sum = scan(n, &upto);
-    if ((unsigned long long)total + sum < 1ull << 31) total += sum; else *bad = true;
+    total = min(total + sum, MAX_LINE);
   }
+  if (total == MAX_LINE) { *bad = true; return false; }
   out->ctas = min(gridDim.x, total);
   if (blockIdx.x >= out->ctas) return false;
   out->share = total / out->ctas;
