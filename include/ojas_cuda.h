@@ -209,9 +209,17 @@ ojc_status ojc_cached_attention_forward(ojc_backend* be, const ojc_tensor* q, co
  * free_pages [F] from entry *free_head on, requests in order, and entered in block_tables (its other entries stay as they are); *free_head_out, another
  * tensor, is the first entry left. Written: starts [B + 1], slots [N], positions [N] (cached length + depth), and masks [N, words] (optional): bit j of
  * row i says that token j of the request is i or an ancestor of i. Rows behind the last token, and tokens without a page, get slot OJC_NONE; the former
- * position 0 and no mask bits. Too few free pages: CapacityExceeded at the next sync. B up to 24,000. */
+ * position 0 and no mask bits. Too few free pages: CapacityExceeded at the next sync. B up to 24,000.
+ * Who holds a page: ojc_paged_plan takes a request for the holder of the pages of its cached places, the first ceil(cached / page) entries of its row, and
+ * of no others. Where the cached length does not grow by all the new tokens (drafts that are rejected), pages entered behind it are lost at the next
+ * plan, which enters others over them, unless the caller returns them to the free pages first. ojc_paged_plan_held keeps them: held_pages [B] says how
+ * many leading entries of its row a request holds (0 for an empty one, at least ceil(cached / page), at most W), these are used before any free
+ * page is taken, and held_pages_out [B], another tensor, is how many it holds now: the next pass's held_pages, whatever became of the drafts. */
 ojc_status ojc_paged_plan(ojc_backend* be, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* parents, const ojc_tensor* free_pages, const ojc_tensor* free_head,
                           int64_t page_size, ojc_tensor* block_tables, ojc_tensor* starts, ojc_tensor* slots, ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out);
+ojc_status ojc_paged_plan_held(ojc_backend* be, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* held_pages, const ojc_tensor* parents,
+                               const ojc_tensor* free_pages, const ojc_tensor* free_head, int64_t page_size, ojc_tensor* block_tables, ojc_tensor* held_pages_out, ojc_tensor* starts,
+                               ojc_tensor* slots, ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out);
 /* Rotary positions without tables: the leading rotary_dim elements of each head are pairs, (i, i + rotary_dim / 2) in the half layout or
  * (2i, 2i + 1) in the interleaved one, and pair i is turned by position * f_i radians and scaled by amplitude; the rest passes through.
  * f_i = base^(-2i / rotary_dim), stretched for contexts beyond original_length: linear f_i / factor; base: base * factor^(R / (R - 2)) for base;

@@ -164,6 +164,7 @@ class PagedPlan:
     positions: Tensor
     masks: Tensor | None
     free_head: Tensor
+    held_pages: Tensor | None = None
 
 
 class CudaBackend:
@@ -482,10 +483,11 @@ class CudaBackend:
     # ---- decode over a paged KV cache
     def paged_plan(self, cached_lens: Tensor, new_lens: Tensor, free_pages: Tensor, free_head: Tensor, block_tables: Tensor, page_size: int, tokens: int | None = None,
                    parents: Tensor | None = None, mask_words: int = 0, starts: Tensor | None = None, slots: Tensor | None = None, positions: Tensor | None = None,
-                   masks: Tensor | None = None, free_head_out: Tensor | None = None) -> PagedPlan:
+                   masks: Tensor | None = None, free_head_out: Tensor | None = None, held_pages: Tensor | None = None, held_pages_out: Tensor | None = None) -> PagedPlan:
         """Plan of a pass over a paged cache (ojc_paged_plan): new tokens `new_lens` [B] behind `cached_lens` [B] get pages from `free_pages` (entered in
         `block_tables` [B, W]), slots and positions, and for trees of drafts ancestor masks of `mask_words` words. `tokens` is the capacity N of the
-        outputs that are not given (by default that of `parents`); rows behind the last token get slot 0xffffffff."""
+        outputs that are not given (by default that of `parents`); rows behind the last token get slot 0xffffffff. `held_pages` [B]: how many entries of its
+        row a request holds, for passes whose drafts may be rejected; the plan's own `held_pages` are the next pass's (ojc_paged_plan_held)."""
         if slots is None and tokens is None:
             if parents is None:
                 raise OjasError(STATUS_NAMES.index("Shape"), "paged_plan: give the capacity `tokens`, `parents` or `slots`")
@@ -497,9 +499,16 @@ class CudaBackend:
         if masks is None and mask_words:
             masks = self.empty((n, mask_words), DType.U32)
         free_head_out = free_head_out if free_head_out is not None else self.empty((1,), DType.U32)
-        _check(lib.ojc_paged_plan(self._handle, _p(cached_lens), _p(new_lens), _p(parents), _p(free_pages), _p(free_head), C.c_int64(page_size), _p(block_tables), _p(starts),
-                                  _p(slots), _p(positions), _p(masks), _p(free_head_out)))
-        return PagedPlan(starts, slots, positions, masks, free_head_out)
+        if held_pages is None:
+            if held_pages_out is not None:
+                raise OjasError(STATUS_NAMES.index("Shape"), "paged_plan: held_pages_out goes with held_pages")
+            _check(lib.ojc_paged_plan(self._handle, _p(cached_lens), _p(new_lens), _p(parents), _p(free_pages), _p(free_head), C.c_int64(page_size), _p(block_tables), _p(starts),
+                                      _p(slots), _p(positions), _p(masks), _p(free_head_out)))
+            return PagedPlan(starts, slots, positions, masks, free_head_out)
+        held_pages_out = held_pages_out if held_pages_out is not None else self.empty(held_pages.shape, DType.U32)
+        _check(lib.ojc_paged_plan_held(self._handle, _p(cached_lens), _p(new_lens), _p(held_pages), _p(parents), _p(free_pages), _p(free_head), C.c_int64(page_size), _p(block_tables),
+                                       _p(held_pages_out), _p(starts), _p(slots), _p(positions), _p(masks), _p(free_head_out)))
+        return PagedPlan(starts, slots, positions, masks, free_head_out, held_pages_out)
 
     @staticmethod
     def rope_plan(spec: RopeSpec) -> "_lib.Rope":

@@ -17,12 +17,13 @@ constexpr int PLAN_THREADS = 256, PLAN_MAX_BATCH = 24000;
 // Every CTA scans the lengths for itself (the running sums stay in its shared memory: one launch, no order between CTAs) and then looks up the
 // request of each of its tokens by bisection. A token's page is either entered already (places below the cached length's last page end) or
 // number `first + page - held` of the free pages, so no CTA reads a table entry that another one writes; the token at a page's first place enters it.
+// `held` is what the cached length needs, or with `held_in` what the request has already been given: pages that drafts took and left again.
 template <int PLAN_TOKENS>
 __global__ void __launch_bounds__(PLAN_THREADS)
-paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restrict__ fresh, const uint32_t* __restrict__ parents, const uint32_t* __restrict__ free_pages,
-                  int64_t n_free, const uint32_t* __restrict__ free_head, uint32_t page, int page_shift, int batch, int64_t width, int64_t tokens, int64_t words,
-                  uint32_t* __restrict__ tables, uint32_t* __restrict__ starts, uint32_t* __restrict__ slots, uint32_t* __restrict__ positions,
-                  uint32_t* __restrict__ masks, uint32_t* __restrict__ head_out, uint32_t* fault) {
+paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restrict__ fresh, const uint32_t* __restrict__ held_in, const uint32_t* __restrict__ parents,
+                  const uint32_t* __restrict__ free_pages, int64_t n_free, const uint32_t* __restrict__ free_head, uint32_t page, int page_shift, int batch, int64_t width, int64_t tokens,
+                  int64_t words, uint32_t* __restrict__ tables, uint32_t* __restrict__ held_out, uint32_t* __restrict__ starts, uint32_t* __restrict__ slots,
+                  uint32_t* __restrict__ positions, uint32_t* __restrict__ masks, uint32_t* __restrict__ head_out, uint32_t* fault) {
   extern __shared__ uint32_t sm[];
   uint32_t* s_start = sm;                  // [batch + 1] first token of each request, clipped to the tokens there is room for
   uint32_t* s_first = sm + batch + 1;      // [batch] free pages taken by the requests before
@@ -31,6 +32,7 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   unsigned long long tok_carry = 0, pg_carry = 0;
   const uint32_t head32 = *free_head;       // asked for before the lengths' scan
   bool bad = false;
+  auto pages = [&](uint32_t x) { const uint32_t q = page_shift >= 0 ? x >> page_shift : x / page; return q + (x != q * page); };
   for (int b0 = 0; b0 < batch; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
     unsigned long long n = 0, g = 0;
@@ -38,8 +40,13 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
       const uint32_t c = cached[b], k = fresh[b], total = c + k;
       n = k;
       bad |= total < c;
-      auto pages = [&](uint32_t x) { const uint32_t q = page_shift >= 0 ? x >> page_shift : x / page; return q + (x != q * page); };
-      g = total < c ? 0 : pages(total) - pages(c);
+      uint32_t held = pages(c);
+      if (held_in) {
+        const uint32_t h = held_in[b];
+        bad |= h < held || h > width;
+        held = max(held, h);
+      }
+      g = total < c || pages(total) < held ? 0 : pages(total) - held;
     }
     unsigned long long tn = n, tg = g;
 #pragma unroll
@@ -65,6 +72,11 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   const unsigned long long head = head32;
   if (blockIdx.x == 0) {
     for (int b = tid; b <= batch; b += PLAN_THREADS) starts[b] = s_start[b];
+    if (held_out) for (int b = tid; b < batch; b += PLAN_THREADS) {       // what is entered: no further than tokens, free pages and the table reach
+      const uint32_t c = cached[b], total = c + (s_start[b + 1] - s_start[b]), held = max(pages(c), held_in[b]);
+      const unsigned long long gone = head + s_first[b], left = gone < (unsigned long long)n_free ? n_free - gone : 0;
+      held_out[b] = max(held, (uint32_t)min((unsigned long long)(total < c ? 0u : pages(total)), min((unsigned long long)held + left, (unsigned long long)width)));
+    }
     if (tid == 0) {
       *head_out = (uint32_t)min(head + pg_carry, max(head, (unsigned long long)n_free));
       if (tok_carry > (unsigned long long)tokens) raise_fault(fault, OP_PAGED_RANGE);
@@ -98,8 +110,8 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
         known = lo;
         first = s_start[lo];
         c = cached[lo];
-        held = page_shift >= 0 ? c >> page_shift : c / page;
-        held += c != held * page;
+        held = pages(c);
+        if (held_in) held = max(held, held_in[lo]);
       }
       const uint32_t local = (uint32_t)t - first, at = c + local;
       const uint32_t pi = page_shift >= 0 ? at >> page_shift : at / page, off = at - pi * page;
@@ -413,6 +425,57 @@ ojc_status rope_run(ojc_backend* be, const char* op, const ojc_rope* rope, const
   });
 }
 
+ojc_status plan_run(ojc_backend* be, const char* op, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* held_pages, const ojc_tensor* parents,
+                    const ojc_tensor* free_pages, const ojc_tensor* free_head, int64_t page_size, ojc_tensor* block_tables, ojc_tensor* held_pages_out, ojc_tensor* starts, ojc_tensor* slots,
+                    ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out) {
+  OJC_ALIVE(be, op);
+  OJC_TRY(u32_vector(op, "cached_lens", cached_lens, -1));
+  const int64_t batch = cached_lens->shape[0];
+  OJC_TRY(u32_vector(op, "new_lens", new_lens, batch));
+  if (held_pages) OJC_TRY(u32_vector(op, "held_pages", held_pages, batch));
+  OJC_TRY(u32_vector(op, "free_pages", free_pages, -1)); OJC_TRY(u32_vector(op, "free_head", free_head, 1));
+  OJC_TRY(u32_vector(op, "starts", starts, batch + 1)); OJC_TRY(u32_vector(op, "slots", slots, -1));
+  const int64_t tokens = slots->shape[0];
+  OJC_TRY(u32_vector(op, "positions", positions, tokens)); OJC_TRY(u32_vector(op, "free_head_out", free_head_out, 1));
+  OJC_TRY(check_tensor(op, "block_tables", block_tables));
+  if (block_tables->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, "block_tables is U32");
+  if (block_tables->rank != 2 || block_tables->shape[0] != batch) return ojc_fail(OJC_ERR_SHAPE, op, "block_tables is [B, W]");
+  if (parents) OJC_TRY(u32_vector(op, "parents", parents, tokens));
+  int64_t words = 0;
+  if (masks) {
+    OJC_TRY(check_tensor(op, "masks", masks));
+    if (masks->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, "masks is U32");
+    if (masks->rank != 2 || masks->shape[0] != tokens || masks->shape[1] == 0) return ojc_fail(OJC_ERR_SHAPE, op, "masks is [N, words]");
+    words = masks->shape[1];
+  }
+  const int64_t width = block_tables->shape[1];
+  if (batch == 0 || tokens == 0 || width == 0) return ojc_fail(OJC_ERR_SHAPE, op, "every dimension must be non-zero");
+  if (batch > PLAN_MAX_BATCH) return ojc_fail(OJC_ERR_UNSUPPORTED, op, "more than 24,000 requests are not supported");
+  if (tokens > INT32_MAX || width > INT32_MAX) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "extent out of range");
+  if (page_size < 1 || page_size > (1 << 24)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "page_size must be in 1..=2^24");
+  if (free_head_out->data == free_head->data) return ojc_fail(OJC_ERR_SHAPE, op, "free_head_out must be another tensor than free_head");
+  OJC_CUDA(be, cudaSetDevice(be->device), op);
+  const size_t smem = (size_t)(2 * batch + 1) * 4;
+  static PerDeviceFlag attr;
+  if (smem > 48 * 1024 - 256 && !attr[be->device]) {
+    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
+    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
+    attr[be->device] = true;
+  }
+  // a token to a thread while that gives every SM a few CTAs at most (trees' chains of parents then run side by side), else four and 16-byte stores
+  const int per_thread = tokens <= (int64_t)be->sm_count * PLAN_THREADS * 4 ? 1 : 4;
+  const int64_t per_cta = PLAN_THREADS * per_thread;
+  const unsigned grid = (unsigned)std::min<int64_t>((tokens + per_cta - 1) / per_cta, (int64_t)be->sm_count * 4);
+  (per_thread == 1 ? paged_plan_kernel<1> : paged_plan_kernel<4>)<<<grid, PLAN_THREADS, smem, be->stream>>>(
+      (const uint32_t*)cached_lens->data, (const uint32_t*)new_lens->data, held_pages ? (const uint32_t*)held_pages->data : nullptr, parents ? (const uint32_t*)parents->data : nullptr,
+      (const uint32_t*)free_pages->data, free_pages->shape[0], (const uint32_t*)free_head->data, (uint32_t)page_size,
+      (page_size & (page_size - 1)) ? -1 : __builtin_ctzll((unsigned long long)page_size), (int)batch, width, tokens, words, (uint32_t*)block_tables->data,
+      held_pages_out ? (uint32_t*)held_pages_out->data : nullptr, (uint32_t*)starts->data, (uint32_t*)slots->data, (uint32_t*)positions->data, masks ? (uint32_t*)masks->data : nullptr,
+      (uint32_t*)free_head_out->data, be->fault_dev);
+  OJC_LAUNCHED(be, op);
+  return OJC_OK;
+}
+
 }  // namespace
 
 ojc_status rope_check(const char* op, const ojc_rope* rope, int64_t head_dim) {
@@ -468,49 +531,16 @@ ojc_status ojc_rope_backward(ojc_backend* be, const ojc_rope* rope, const ojc_te
 
 ojc_status ojc_paged_plan(ojc_backend* be, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* parents, const ojc_tensor* free_pages, const ojc_tensor* free_head,
                           int64_t page_size, ojc_tensor* block_tables, ojc_tensor* starts, ojc_tensor* slots, ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out) {
-  const char* op = "paged_plan";
+  return plan_run(be, "paged_plan", cached_lens, new_lens, nullptr, parents, free_pages, free_head, page_size, block_tables, nullptr, starts, slots, positions, masks, free_head_out);
+}
+ojc_status ojc_paged_plan_held(ojc_backend* be, const ojc_tensor* cached_lens, const ojc_tensor* new_lens, const ojc_tensor* held_pages, const ojc_tensor* parents,
+                               const ojc_tensor* free_pages, const ojc_tensor* free_head, int64_t page_size, ojc_tensor* block_tables, ojc_tensor* held_pages_out, ojc_tensor* starts,
+                               ojc_tensor* slots, ojc_tensor* positions, ojc_tensor* masks, ojc_tensor* free_head_out) {
+  const char* op = "paged_plan_held";
   OJC_ALIVE(be, op);
-  OJC_TRY(u32_vector(op, "cached_lens", cached_lens, -1));
-  const int64_t batch = cached_lens->shape[0];
-  OJC_TRY(u32_vector(op, "new_lens", new_lens, batch)); OJC_TRY(u32_vector(op, "free_pages", free_pages, -1)); OJC_TRY(u32_vector(op, "free_head", free_head, 1));
-  OJC_TRY(u32_vector(op, "starts", starts, batch + 1)); OJC_TRY(u32_vector(op, "slots", slots, -1));
-  const int64_t tokens = slots->shape[0];
-  OJC_TRY(u32_vector(op, "positions", positions, tokens)); OJC_TRY(u32_vector(op, "free_head_out", free_head_out, 1));
-  OJC_TRY(check_tensor(op, "block_tables", block_tables));
-  if (block_tables->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, "block_tables is U32");
-  if (block_tables->rank != 2 || block_tables->shape[0] != batch) return ojc_fail(OJC_ERR_SHAPE, op, "block_tables is [B, W]");
-  if (parents) OJC_TRY(u32_vector(op, "parents", parents, tokens));
-  int64_t words = 0;
-  if (masks) {
-    OJC_TRY(check_tensor(op, "masks", masks));
-    if (masks->dtype != OJC_U32) return ojc_fail(OJC_ERR_DTYPE, op, "masks is U32");
-    if (masks->rank != 2 || masks->shape[0] != tokens || masks->shape[1] == 0) return ojc_fail(OJC_ERR_SHAPE, op, "masks is [N, words]");
-    words = masks->shape[1];
-  }
-  const int64_t width = block_tables->shape[1];
-  if (batch == 0 || tokens == 0 || width == 0) return ojc_fail(OJC_ERR_SHAPE, op, "every dimension must be non-zero");
-  if (batch > PLAN_MAX_BATCH) return ojc_fail(OJC_ERR_UNSUPPORTED, op, "more than 24,000 requests are not supported");
-  if (tokens > INT32_MAX || width > INT32_MAX) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "extent out of range");
-  if (page_size < 1 || page_size > (1 << 24)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "page_size must be in 1..=2^24");
-  if (free_head_out->data == free_head->data) return ojc_fail(OJC_ERR_SHAPE, op, "free_head_out must be another tensor than free_head");
-  OJC_CUDA(be, cudaSetDevice(be->device), op);
-  const size_t smem = (size_t)(2 * batch + 1) * 4;
-  static PerDeviceFlag attr;
-  if (smem > 48 * 1024 - 256 && !attr[be->device]) {
-    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
-    OJC_CUDA(be, cudaFuncSetAttribute(paged_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * PLAN_MAX_BATCH + 1) * 4), op);
-    attr[be->device] = true;
-  }
-  // a token to a thread while that gives every SM a few CTAs at most (trees' chains of parents then run side by side), else four and 16-byte stores
-  const int per_thread = tokens <= (int64_t)be->sm_count * PLAN_THREADS * 4 ? 1 : 4;
-  const int64_t per_cta = PLAN_THREADS * per_thread;
-  const unsigned grid = (unsigned)std::min<int64_t>((tokens + per_cta - 1) / per_cta, (int64_t)be->sm_count * 4);
-  (per_thread == 1 ? paged_plan_kernel<1> : paged_plan_kernel<4>)<<<grid, PLAN_THREADS, smem, be->stream>>>(
-      (const uint32_t*)cached_lens->data, (const uint32_t*)new_lens->data, parents ? (const uint32_t*)parents->data : nullptr, (const uint32_t*)free_pages->data,
-      free_pages->shape[0], (const uint32_t*)free_head->data, (uint32_t)page_size, (page_size & (page_size - 1)) ? -1 : __builtin_ctzll((unsigned long long)page_size), (int)batch, width, tokens, words, (uint32_t*)block_tables->data, (uint32_t*)starts->data,
-      (uint32_t*)slots->data, (uint32_t*)positions->data, masks ? (uint32_t*)masks->data : nullptr, (uint32_t*)free_head_out->data, be->fault_dev);
-  OJC_LAUNCHED(be, op);
-  return OJC_OK;
+  OJC_TRY(u32_vector(op, "held_pages", held_pages, -1)); OJC_TRY(u32_vector(op, "held_pages_out", held_pages_out, held_pages->shape[0]));
+  if (held_pages_out->data == held_pages->data) return ojc_fail(OJC_ERR_SHAPE, op, "held_pages_out must be another tensor than held_pages");
+  return plan_run(be, op, cached_lens, new_lens, held_pages, parents, free_pages, free_head, page_size, block_tables, held_pages_out, starts, slots, positions, masks, free_head_out);
 }
 
 ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* v_pages, const ojc_tensor* k, const ojc_tensor* v, const ojc_tensor* slots, const ojc_rope* rope,

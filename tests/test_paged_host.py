@@ -183,3 +183,24 @@ def test_a_changed_tensor_is_passed_as_it_is_now():
     assert _p(x)._obj.data == 256 and _p(x) is _p(x)
     x.ptr, x.shape, x.strides = 512, (5, 2, 32), (128, 64, 1)
     assert _p(x)._obj.data == 512 and list(_p(x)._obj.shape[:3]) == [5, 2, 32] and list(_p(x)._obj.stride[:3]) == [128, 64, 1]
+
+
+def test_paged_plan_held_refusals(handle):
+    u32 = DType.U32
+
+    def run(held, out, batch=3):
+        a = [t((3,), u32), t((3,), u32), held, None, t((9,), u32), t((1,), u32)]
+        return kind(lib.ojc_paged_plan_held(handle, *[_p(x) for x in a], C.c_int64(16), _p(t((batch, 4), u32)), _p(out), _p(t((4,), u32)), _p(t((10,), u32)), _p(t((10,), u32)), None,
+                                            _p(t((1,), u32, ptr=512))))
+    good = t((3,), u32, ptr=1024)
+    assert run(None, good) == "Shape" and run(good, None) == "Shape"
+    assert run(t((3,)), good) == "Dtype" and run(t((3,), u32), t((3,), ptr=1024)) == "Dtype"
+    assert run(t((2,), u32), t((2,), u32, ptr=1024)) == "Shape" and run(t((3,), u32), t((4,), u32, ptr=1024)) == "Shape" and run(t((3, 1), u32), good) == "Shape"
+    assert run(good, t((3,), u32, ptr=1024)) == "Shape" and "another tensor" in lib.ojc_last_error().decode()
+    assert run(t((3,), u32), good, batch=2) == "Shape"
+    assert kind(lib.ojc_paged_plan_held(*([None] * 7), C.c_int64(16), *([None] * 7))) == "Backend"
+    be = CudaBackend.__new__(CudaBackend)
+    be._handle = None
+    with pytest.raises(OjasError) as e:
+        be.paged_plan(*[t((3,), u32)] * 4, t((3, 4), u32), 16, tokens=4, starts=t((4,), u32), slots=t((4,), u32), positions=t((4,), u32), free_head_out=t((1,), u32), held_pages_out=good)
+    assert e.value.kind == "Shape"
