@@ -122,7 +122,7 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
         else if (pi < held) { id = tables[(int64_t)lo * width + pi]; bad |= id == 0xffffffffull; }
         else {
           const unsigned long long e = head + s_first[lo] + (pi - held);
-          if (e < (unsigned long long)n_free) id = free_pages[e];
+          if (e < (unsigned long long)n_free) { id = free_pages[e]; bad |= id == 0xffffffffull; }
         }
       }
       if (off == 0 && pi >= held && id != 0xffffffffull) tables[(int64_t)lo * width + pi] = (uint32_t)id;

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_paged import be, floats, u32  # noqa: F401  (be: the module's backend)
+from test_gpu_paged import NONE, be, floats, u32  # noqa: F401  (be: the module's backend)
 
 pytestmark = pytest.mark.gpu
 
@@ -59,7 +59,7 @@ def test_pages_of_rejected_drafts_stay_with_their_request(be, page, batch):
         n = sum(row) + 2
         want, head, held, tables = held_plan(cached, row, held, free, head, tables, page)
         got = be.paged_plan(u32(be, cached), u32(be, row), d_free, d_head, d_tables, page, tokens=n, held_pages=d_held)
-        assert list(got.slots.numpy()) == want + [0xFFFFFFFF] * 2 and list(got.held_pages.numpy()) == held and got.free_head.numpy()[0] == head
+        assert list(got.slots.numpy()) == want + [NONE] * 2 and list(got.held_pages.numpy()) == held and got.free_head.numpy()[0] == head
         d_head, d_held = got.free_head, got.held_pages
         cached += keep
     be.sync()
@@ -97,3 +97,13 @@ def test_held_pages_are_those_that_were_entered(be, what, kind, held_after):
         for i in range(width):
             before = max(held[b], -(-cached[b] // 4))
             assert (entered[b, i] == tables[b, i]) == (i < before or i >= held_after[b])
+
+
+def test_a_free_entry_that_names_no_page_is_reported(be):
+    from ojas_b200 import OjasError
+    tables, free = u32(be, np.full((2, 4), 9)), u32(be, [3, NONE, 5])
+    got = be.paged_plan(u32(be, [0, 0]), u32(be, [8, 3]), free, u32(be, [0]), tables, 4, tokens=11)
+    with pytest.raises(OjasError) as e:
+        be.sync()
+    assert e.value.kind == "OutOfRange"
+    assert list(got.slots.numpy()) == [12, 13, 14, 15, NONE, NONE, NONE, NONE, 20, 21, 22] and tables.numpy()[1, 0] == 5
