@@ -26,7 +26,7 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
                   uint32_t* __restrict__ positions, uint32_t* __restrict__ masks, uint32_t* __restrict__ head_out, uint32_t* fault) {
   extern __shared__ uint32_t sm[];
   uint32_t* s_start = sm;                  // [batch + 1] first token of each request, clipped to the tokens there is room for
-  uint32_t* s_first = sm + batch + 1;      // [batch] free pages taken by the requests before
+  uint32_t* s_first = sm + batch + 1;      // [batch] free pages taken by the requests before; all ones: none is for this request
   __shared__ unsigned long long w_tok[PLAN_THREADS / 32], w_pg[PLAN_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned long long tok_carry = 0, pg_carry = 0;
@@ -36,17 +36,19 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
   for (int b0 = 0; b0 < batch; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
     unsigned long long n = 0, g = 0;
+    bool passes = false;                     // its places pass 32 bits: no token of it gets a slot, and it takes no page
     if (b < batch) {
       const uint32_t c = cached[b], k = fresh[b], total = c + k;
       n = k;
-      bad |= total < c;
+      passes = total < c;
+      bad |= passes;
       uint32_t held = pages(c);
       if (held_in) {
         const uint32_t h = held_in[b];
         bad |= h < held || h > width;
         held = max(held, h);
       }
-      g = total < c || pages(total) < held ? 0 : pages(total) - held;
+      g = passes || pages(total) < held ? 0 : pages(total) - held;
     }
     unsigned long long tn = n, tg = g;
 #pragma unroll
@@ -64,7 +66,7 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
     }
     if (b < batch) {
       s_start[b] = (uint32_t)min(before_t + tn - n, (unsigned long long)tokens);
-      s_first[b] = (uint32_t)min(before_g + tg - g, 0xffffffffull);
+      s_first[b] = passes ? 0xffffffffu : (uint32_t)min(before_g + tg - g, 0xffffffffull);
     }
   }
   if (tid == 0) s_start[batch] = (uint32_t)min(tok_carry, (unsigned long long)tokens);
@@ -119,10 +121,12 @@ paged_plan_kernel(const uint32_t* __restrict__ cached, const uint32_t* __restric
         known_page = pi;
         id = 0xffffffffull;
         if (pi >= width) bad = true;
-        else if (pi < held) { id = tables[(int64_t)lo * width + pi]; bad |= id == 0xffffffffull; }
-        else {
-          const unsigned long long e = head + s_first[lo] + (pi - held);
-          if (e < (unsigned long long)n_free) { id = free_pages[e]; bad |= id == 0xffffffffull; }
+        else if (s_first[lo] != 0xffffffffu) {
+          if (pi < held) { id = tables[(int64_t)lo * width + pi]; bad |= id == 0xffffffffull; }
+          else {
+            const unsigned long long e = head + s_first[lo] + (pi - held);
+            if (e < (unsigned long long)n_free) { id = free_pages[e]; bad |= id == 0xffffffffull; }
+          }
         }
       }
       if (off == 0 && pi >= held && id != 0xffffffffull) tables[(int64_t)lo * width + pi] = (uint32_t)id;

@@ -107,3 +107,18 @@ def test_a_free_entry_that_names_no_page_is_reported(be):
         be.sync()
     assert e.value.kind == "OutOfRange"
     assert list(got.slots.numpy()) == [12, 13, 14, 15, NONE, NONE, NONE, NONE, 20, 21, 22] and tables.numpy()[1, 0] == 5
+
+
+def test_a_length_that_passes_32_bits_takes_no_page(be):
+    """Request 0's lengths add up to more than 32 bits hold: none of its tokens gets a slot, request 1's page is its own."""
+    from ojas_b200 import OjasError
+    page = 1 << 24
+    new = [page + 6, 2]
+    tables = u32(be, np.zeros((2, 256)))
+    got = be.paged_plan(u32(be, [(1 << 32) - page - 3, 0]), u32(be, new), u32(be, [77, 78]), u32(be, [0]), tables, page, tokens=sum(new))
+    with pytest.raises(OjasError) as e:
+        be.sync()
+    assert e.value.kind == "OutOfRange"
+    slots, entered = got.slots.numpy(), tables.numpy()
+    assert np.all(slots[: new[0]] == NONE) and list(slots[new[0]:]) == [77 * page, 77 * page + 1]
+    assert entered[1, 0] == 77 and not entered[0].any() and got.free_head.numpy()[0] == 1
