@@ -244,8 +244,9 @@ ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* 
  * Head h reads KV head h / (H / Hkv), the scale is 1 / sqrt(D). Token i of request b sees the cached places below cached_lens[b] and, of the
  * request's new tokens, those whose bits are set in row i of masks [N, words], or without masks those up to itself; of all these, with window >= 1,
  * only those whose position is above its own minus window (the position of a cached place is the place, that of a new token its entry of positions
- * [N], at least the cached length; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). Masked places are never
- * looked at: NaN or infinity there does no harm. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
+ * [N], at least the cached length; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). What
+ * masked places hold is never looked at: NaN or infinity there does no harm. Entries of block_tables for pages wholly before place cached_lens[b] -
+ * window + 1 are not read, so such pages may have been released; from there to the request's last token every entry has to name a page. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
  * non-finite value that a row does see surfaces as NonFinite. A call with 2^31 - 1 blocks of 64 or 128 keys or more, over all row tiles and KV heads,
  * computes nothing and surfaces as OutOfRange. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
  * NULL for the library's own (refused while the stream is being captured). */

@@ -187,14 +187,15 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   Cursor<BLOCK_KEYS> ahead = use;                                                                                   // the block whose pages are looked up next
 
   // ---- copies: warp w fetches WARP_KEYS keys of a block from number w * WARP_KEYS on; with 16, lane l looks up key l's row of K and lane 16 + l its row of V,
-  // with 32 a lane does both. Places behind the last one repeat it: what lies there is masked like any place that is not seen.
+  // with 32 a lane does both. Places behind the last one repeat it, those before the first that a row can see repeat that one: what lies there is masked like any place that is not seen.
   const PagesView<const T>& mine = lane < 16 ? kp : vp;
   const char* const mine_ptr = (const char*)mine.ptr;
   const int64_t mine_sp = mine.sp * (int)sizeof(T), mine_st = mine.st * (int)sizeof(T), mine_sh = mine.sh * (int)sizeof(T);
   struct Place { uint32_t id, off; int hk; };
   auto look_up = [&]() {
     Place p;
-    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + WARP_KEYS * warp + lane % WARP_KEYS), last);
+    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1;
+    const uint32_t j = max(min((uint32_t)((ahead.r.first_block + ahead.block) * BLOCK_KEYS + WARP_KEYS * warp + lane % WARP_KEYS), last), first_place(ix, ahead.r.cached));
     const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
     p.off = j - pi * ix.page;
     p.id = ix.tables[(int64_t)ahead.b * ix.width + pi];
@@ -619,11 +620,13 @@ paged_attention_few_kernel(RowsView<const float> q, PagesView<const float> kp, P
   const uint32_t begin = share.begin;
   const int todo = share.todo;
   Cursor<KEYS> use = share.at, ahead = use;
-  // copies: lane l looks up key l's row of K, lane 16 + l its row of V; places behind the last one repeat it
+  // copies: lane l looks up key l's row of K, lane 16 + l its row of V; places behind the last one repeat it, those before the first
+  // that a row can see repeat that one
   struct Place { uint32_t id, off; int hk; };
   auto look_up = [&]() {
     Place p;
-    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1, j = min((uint32_t)((ahead.r.first_block + ahead.block) * KEYS + 16 * warp + (lane & 15)), last);
+    const uint32_t last = ahead.r.cached + (uint32_t)ahead.r.fresh - 1;
+    const uint32_t j = max(min((uint32_t)((ahead.r.first_block + ahead.block) * KEYS + 16 * warp + (lane & 15)), last), first_place(ix, ahead.r.cached));
     const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
     p.off = j - pi * ix.page;
     p.id = ix.tables[(int64_t)ahead.b * ix.width + pi];

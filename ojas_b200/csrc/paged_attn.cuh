@@ -50,6 +50,10 @@ __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.f
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 constexpr float LOG2_E = 1.4426950408889634f, LN_2 = 0.6931471805599453f;
 
+// The first place that a row of the request can see (positions of new tokens are at least `cached`). Pages that lie wholly before it are never looked up:
+// their entries may name no page any more.
+__device__ __forceinline__ uint32_t first_place(const PassIndex& ix, uint32_t cached) { return ix.window > 0 && cached >= ix.window ? cached - (uint32_t)ix.window + 1 : 0; }
+
 struct Request { uint32_t cached, first; int fresh, first_block, blocks, row_tiles; };
 template <int KEYS>
 __device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int group, int tile_rows, bool* bad) {
@@ -60,8 +64,7 @@ __device__ __forceinline__ Request load_request(const PassIndex& ix, int b, int 
   r.cached = wrong ? 0 : cached;
   r.first = first;
   r.fresh = wrong ? 0 : (int)(end - first);
-  const int64_t from = ix.window > 0 ? (int64_t)r.cached - ix.window + 1 : 0;   // positions of new tokens are at least `cached`
-  r.first_block = from > 0 ? (int)(from / KEYS) : 0;
+  r.first_block = (int)(first_place(ix, r.cached) / KEYS);
   r.blocks = r.fresh == 0 ? 0 : (int)((r.cached + (uint32_t)r.fresh + KEYS - 1) / KEYS) - r.first_block;
   r.row_tiles = (int)((uint32_t)(r.fresh * group + tile_rows - 1) / (uint32_t)tile_rows);
   return r;

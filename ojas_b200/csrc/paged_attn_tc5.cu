@@ -16,9 +16,9 @@
 // What bounds it: with one tile of 64 rows or so the cache's bytes (64 KB of K and V per block and SM); with two tiles the exponentials: 128 x 128 per
 // block and tile at 16 a cycle and SM take 1024 cycles, the two products 512.
 //
-// V's rows behind a request's last place are whatever the page held: the softmax threads overwrite them with zeros before P V reads them. A place that
-// some rows see and others do not may hold NaN or infinity: the blocks with masks are searched for such values; where there are any, each row adds its
-// own share of them to O by itself and the operand's are replaced by zeros.
+// V's rows behind a request's last place are whatever the page held, and no box is fetched for pages before its first one: the softmax threads overwrite
+// all those rows with zeros before P V reads them. A place that some rows see and others do not may hold NaN or infinity: the blocks with masks are
+// searched for such values; where there are any, each row adds its own share of them to O by itself and the operand's are replaced by zeros.
 // Every mbarrier wait is bounded; on expiry the CTA raises the fault word, drains and frees its TMEM.
 #include "paged_attn.cuh"
 #include "tc_common.cuh"
@@ -181,7 +181,7 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
     bool there = false;
     auto look_up = [&]() {
       const uint32_t last = use.r.cached + (uint32_t)use.r.fresh - 1, j = (uint32_t)(use.r.first_block + use.block) * KEYS + lane * pg;
-      there = lane * pg < KEYS && j <= last;
+      there = lane * pg < KEYS && j <= last && j + pg > first_place(ix, use.r.cached);
       if (there) {
         const uint32_t pi = ix.page_shift >= 0 ? j >> ix.page_shift : j / ix.page;
         off = j - pi * ix.page;
@@ -353,16 +353,16 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
       uint32_t bits[4];
       if (masked) {
         seen_bits(ix, use.r, row, j0, bits);
-        // V's rows behind the last place become zeros; the others are searched for values that are not finite
+        // V's rows behind the last place, and those before the first that a row can see, become zeros; the others are searched for values that are not finite
         if (!mbar_wait(bar(C::VFULL + stage), (f / STAGES) & 1, fault, abort_flag)) { ok = false; break; }
         uint32_t odd = 0;
+        const bool outside = j0 + t >= places || j0 + t < first_place(ix, use.r.cached);
         for (int part = g; part < C::NSUB; part += T) {           // T 2 and one sub-tile: the first tile's threads do it all
           uint8_t* v = smem_raw + C::OFF_V + stage * C::TILE_BYTES + part * SUB_BYTES + t * 128;
-          const bool behind = j0 + t >= places;
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             uint4* w = reinterpret_cast<uint4*>(v + ((c ^ (t & 7)) << 4));
-            if (behind) *w = make_uint4(0, 0, 0, 0);
+            if (outside) *w = make_uint4(0, 0, 0, 0);
             else {
               const uint4 x = *w;
               const uint32_t u[4] = {x.x, x.y, x.z, x.w};

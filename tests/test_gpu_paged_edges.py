@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_paged import NONE, be, floats, u32  # noqa: F401  (be: the module's backend)
+from test_gpu_paged import NONE, Case, be, floats, u32  # noqa: F401  (be: the module's backend)
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,40 @@ def test_a_length_that_passes_32_bits_takes_no_page(be):
     slots, entered = got.slots.numpy(), tables.numpy()
     assert np.all(slots[: new[0]] == NONE) and list(slots[new[0]:]) == [77 * page, 77 * page + 1]
     assert entered[1, 0] == 77 and not entered[0].any() and got.free_head.numpy()[0] == 1
+
+
+# one shape for each kernel: cached, new, heads, KV heads, dim, page, BF16
+KERNELS = {"rows": ([300, 77], [3, 1], 4, 2, 40, 8, True), "few f32": ([700, 90], [1, 1], 4, 2, 64, 16, False), "tiles f32": ([500, 131], [9, 4], 4, 2, 96, 8, False),
+           "tiles of 16": ([900, 200], [3, 1], 8, 2, 128, 16, True), "tiles of 16, 128 keys": ([900, 200], [3, 1], 8, 2, 64, 8, True), "tiles of 32": ([500, 77], [12, 9], 4, 2, 64, 24, True),
+           "tiles of 64": ([500, 77], [20, 30], 2, 1, 80, 20, True), "tiles of 192 columns": ([300, 170], [2, 9], 4, 1, 192, 16, True),
+           "tcgen05": ([700, 150], [40, 35], 4, 4, 64, 16, True), "tcgen05, two tiles": ([900, 150], [150, 135], 4, 2, 128, 8, True),
+           "tcgen05, large pages": ([900, 700], [60, 64], 2, 2, 128, 256, True)}
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("window", [1, 5, 70, 200])
+@pytest.mark.parametrize("tree", [True, False])
+def test_pages_before_the_window_may_be_released(be, kernel, window, tree):
+    """Entries of pages that lie wholly before the request's first visible place, cached - window + 1, name no page any more: the same bits, no fault."""
+    cached, new, h, hk, d, page, bf16 = KERNELS[kernel]
+    c = Case(70 + window, cached, new, h, hk, d, page, tree, bf16)
+    out, lse = c.check(be, window=window)
+    for b in range(len(cached)):
+        c.tables[b, : max(0, cached[b] - window + 1) // page] = NONE
+    for kw in (dict(), dict(heads_first=True)):
+        got = c.run(be, window=window, **kw)
+        assert np.array_equal(got[0], out) and np.array_equal(got[1], lse)
+    if not tree:
+        got = c.run(be, window=window, use_positions=False)
+        assert np.array_equal(got[0], out) and np.array_equal(got[1], lse)
+
+
+def test_the_page_of_the_first_visible_place_is_still_followed(be):
+    from ojas_b200 import OjasError
+    for kernel in KERNELS:
+        cached, new, h, hk, d, page, bf16 = KERNELS[kernel]
+        c = Case(71, cached, new, h, hk, d, page, False, bf16)
+        c.tables[0, (cached[0] - 40 + 1) // page] = NONE
+        with pytest.raises(OjasError) as e:
+            c.run(be, window=40)
+        assert e.value.kind == "OutOfRange", kernel
