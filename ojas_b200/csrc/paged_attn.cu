@@ -111,7 +111,8 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 // What bounds it: the cache's bytes for few rows. Four warps to a CTA, one to three CTAs to an SM, two or three stages of 64 or 128 keys each, rows fetched by 16-byte asynchronous
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
-// Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is dropped is 2^-22 of a product).
+// Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is
+// dropped is 2^-22 of a product, 2^-21 of a weight times a value).
 constexpr int TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -135,6 +136,12 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
 // x = hi + lo up to 2^-22 |x|, both TF32
 __device__ __forceinline__ void split_tf32(float x, uint32_t* hi, uint32_t* lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*lo) : "f"(x - __uint_as_float(*hi)));
+}
+// The same for a value, its upper half cut off and not rounded: a finite one stays finite (the last binade would round up to infinity). x = hi + lo up to
+// 2^-21 |x|; errors of the outputs are the same, and the cut is cheaper than the conversion (which saturated takes 7 % of the kernel).
+__device__ __forceinline__ void split_tf32_value(float x, uint32_t* hi, uint32_t* lo) {
+  *hi = __float_as_uint(x) & 0xffffe000u;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*lo) : "f"(x - __uint_as_float(*hi)));
 }
 __device__ __forceinline__ float quad_max(float v) { v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1)); return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)); }
@@ -360,6 +367,33 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
           for (int e = 0; e < 4; ++e) s[n][e] += s1[APART ? n : 0][e] + s2[APART ? n : 0][e];
         }
       }
+      // An operand that is infinite, or rounds up to it, is not the sum of its two parts: scores that are not finite are formed once more from the operands
+      float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd[e] = fmaf(s[n][e], 0.0f, odd[e]);
+      }
+      if (__any_sync(0xffffffffu, (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.0f)) {
+#pragma unroll 1
+        for (int n = 0; n < NT; ++n) {                                                                  // the tile in work is s[0]: they move on
+          float now[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float* qr = reinterpret_cast<const float*>(q_tile) + (16 * mw + quad + 8 * (e >> 1)) * S::K_PITCH;
+            const float* kr = reinterpret_cast<const float*>(kt) + (8 * n + 2 * pair + (e & 1)) * S::K_PITCH;
+            now[e] = s[0][e];
+            if (!isfinite(now[e])) {
+              now[e] = 0.0f;
+#pragma unroll 1
+              for (int d = 0; d < D; ++d) now[e] = fmaf(qr[d], kr[d], now[e]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i + 1 < NT; ++i) { s[i][0] = s[i + 1][0]; s[i][1] = s[i + 1][1]; s[i][2] = s[i + 1][2]; s[i][3] = s[i + 1][3]; }
+          s[NT - 1][0] = now[0]; s[NT - 1][1] = now[1]; s[NT - 1][2] = now[2]; s[NT - 1][3] = now[3];
+        }
+      }
     }
 
     // ---- what the rows see: everything in a block below the cached length and inside every row's window
@@ -472,7 +506,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
 #pragma unroll
         for (int n = 0; n < OT; ++n) {
           uint32_t bh0, bl0, bh1, bl1;
-          split_tf32(va[k * 8 * S::V_PITCH + 8 * n], &bh0, &bl0); split_tf32(va[(k * 8 + 1) * S::V_PITCH + 8 * n], &bh1, &bl1);
+          split_tf32_value(va[k * 8 * S::V_PITCH + 8 * n], &bh0, &bl0); split_tf32_value(va[(k * 8 + 1) * S::V_PITCH + 8 * n], &bh1, &bl1);
           mma_tf32(o[n], al, bh0, bh1);
           mma_tf32(o[n], ah, bl0, bl1);
           mma_tf32(o[n], ah, bh0, bh1);

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_paged import NONE, Case, be, floats, u32  # noqa: F401  (be: the module's backend)
+from test_gpu_paged import HALF_BF16, HALF_F32, NONE, Case, be, floats, u32  # noqa: F401  (be: the module's backend)
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,54 @@ def test_the_page_of_the_first_visible_place_is_still_followed(be):
         with pytest.raises(OjasError) as e:
             c.run(be, window=40)
         assert e.value.kind == "OutOfRange", kernel
+
+
+def scored_minus_infinity(c, drop):
+    """The case's reference where the places of `drop` (request 0) score -inf in every row that sees them: they weigh nothing."""
+    keep_k, keep_v = c.k.copy(), c.v.copy()
+    for p in drop:
+        page, off = c.slot(0, p)
+        c.k[page, off, :, 0] = -np.inf
+    n, d, h, hk = int(c.starts[-1]), c.q.shape[2], c.q.shape[1], c.k.shape[2]
+    out, lse, tol, lse_tol = np.zeros((n, h, d)), np.full((n, h), np.nan), np.zeros((n, h, d)), np.zeros((n, h))
+    half, eps_p = (HALF_BF16, HALF_BF16) if c.bf16 else (HALF_F32, 0.0)
+    cached, total = int(c.cached[0]), int(c.cached[0] + c.new[0])
+    at = np.arange(total)
+    k, v = (a[c.tables[0, at // c.page], at % c.page].astype(np.float64) for a in (keep_k, keep_v))
+    for t in range(n):
+        sees = at <= cached + t
+        if c.masks is not None:
+            sees = np.array([p < cached or bool(c.masks[t, (p - cached) // 32] >> np.uint32((p - cached) % 32) & 1) for p in at])
+        sees[list(drop)] = False
+        for head in range(h):
+            kk, vv = k[sees, head // (h // hk)], v[sees, head // (h // hk)]
+            if not len(kk):
+                out[t, head] = np.nan
+                continue
+            s = kk @ c.q[t, head].astype(np.float64) / np.sqrt(d)
+            p = np.exp(s - s.max())
+            lse[t, head], out[t, head] = s.max() + np.log(p.sum()), p @ vv / p.sum()
+            e_s = (d + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(c.q[t, head])).max() / np.sqrt(d)
+            e_w = e_s + 2.0 ** -20 + (total + 8) * 2.0 ** -24                      # as in paged_reference.attention
+            tol[t, head] = (half + 2.0 ** -22) * np.abs(out[t, head]) + (2 * e_w + eps_p * (1 + 2.0 ** -6)) * (p @ np.abs(vv) / p.sum()) * (1 + half) + 1e-30
+            lse_tol[t, head] = e_w + e_s + 2.0 ** -22 * (1 + abs(lse[t, head]))
+    return out, lse, tol, lse_tol
+
+
+@pytest.mark.parametrize("h,hk,d,cached,new", [(8, 1, 96, 9, 1), (4, 1, 64, 6, 2), (16, 1, 128, 7, 3), (8, 1, 32, 300, 10)])
+def test_f32_operands_at_the_ends_of_the_range(be, h, hk, d, cached, new):
+    """The tiles take an F32 operand apart into two of fewer bits: a key's infinity gives the infinite score, and what would round up to an infinity stays
+    finite. The largest values are 2^128 - 2^116: the sums' rounding, 2^-20 of them and less, stays below the 2^-12 that are left."""
+    big = np.float32(2.0 ** 128 - 2.0 ** 116)
+    c = Case(73, [cached], [new], h, hk, d, 16, True, False)
+    c.q[..., 0] = 1.0
+    want, want_lse, tol, lse_tol = scored_minus_infinity(c, [cached])
+    assert np.any(np.isinf(c.k))
+    got, lse = c.run(be)
+    assert np.all(np.abs(got - want) <= tol) and np.all(np.abs(lse - want_lse) <= lse_tol)
+    c = Case(74, [cached], [new], h, hk, d, 16, True, False)
+    c.k[..., 1], c.q[..., 1] = big, 2.0 ** -126
+    first, off = c.slot(0, 0)
+    c.v[first, off, :, 2], c.v[first, off, :, 3] = -0.5 * big, big              # at one place: the running sums are not normalised
+    got, lse = c.check(be)
+    assert np.all(np.isfinite(got))
