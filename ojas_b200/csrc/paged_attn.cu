@@ -77,9 +77,8 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
     if (seen == 0) continue;
     any = true;
     const float m_new = fmaxf(m, warp_max(s));
-    // every score -inf so far (or NaN among them): the sum shows it below
-    const float corr = m_new == -INFINITY ? 1.0f : expf(m - m_new);
-    const float p = sees ? expf(s - m_new) : 0.0f;
+    const float base = m_new == -INFINITY ? 0.0f : m_new;      // every score -inf so far
+    const float corr = expf(m - base), p = sees ? expf(s - base) : 0.0f;
     l = l * corr + warp_sum(p);
 #pragma unroll
     for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) o[i] *= corr;
@@ -93,7 +92,8 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
     m = m_new;
   }
   bool wrong = any && !(isfinite(l) && l > 0.0f && isfinite(m));
-  const float inv = any ? 1.0f / l : 0.0f;
+  l = only_minus_inf(any, m, l);
+  const float inv = inverse_sum(m, l);
   T* po = out.ptr + t * out.sn + h * out.sh;
 #pragma unroll
   for (int i = 0; i < MAX_HEAD_COLUMNS; ++i) {
@@ -522,7 +522,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
         l[x] = quad_sum(l[x]);
         int seen = any[x];
         seen |= __shfl_xor_sync(0xffffffffu, seen, 1); seen |= __shfl_xor_sync(0xffffffffu, seen, 2);
-        if (seen && m[x] == -INFINITY) l[x] = NAN;                                                      // every score -inf: what the formula gives
+        l[x] = only_minus_inf(seen, m[x], l[x]);
       }
       if (KW > 1) {                                                                                     // the warps that share a row tile add up in order
         const int rows = min(16, use.r.fresh * group - row_tile * TILE_ROWS);                            // of a row tile of 16 (MW 1)
@@ -545,7 +545,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
             if (!live[x]) continue;
             const float m2 = jm[2 * r], l2 = jm[2 * r + 1], top = fmaxf(m[x], m2), base = top == -INFINITY ? 0.0f : top * c2;
             const float ca = exp2_fast(fmaf(m[x], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
-            l[x] = l[x] * ca + l2 * cb;
+            l[x] = joined_sum(top, l[x], ca, l2, cb);
             m[x] = top;
 #pragma unroll
             for (int n = 0; n < OT; ++n) {
@@ -588,7 +588,7 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
           const int h = hk * group + r % group;
           if (whole) {
             const bool seen = !(m[x] == -INFINITY && l[x] == 0.0f);
-            const float inv = seen ? 1.0f / l[x] : 0.0f;
+            const float inv = inverse_sum(m[x], l[x]);
             T* p = out.ptr + t * out.sn + h * out.sh;
 #pragma unroll
             for (int n = 0; n < OT; ++n) {
@@ -803,7 +803,7 @@ paged_attention_few_kernel(RowsView<const float> q, PagesView<const float> kp, P
     const bool unit_done = use.block + 1 == use.r.blocks;
     if (unit_done || f + 1 == todo) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) if (any[r] && m[r] == -INFINITY) l[r] = NAN;     // every score -inf: what the formula gives
+      for (int r = 0; r < R; ++r) l[r] = only_minus_inf(any[r], m[r], l[r]);
       __syncthreads();                                                          // what a unit before left has been taken
       if (warp > 0) {
 #pragma unroll
@@ -826,7 +826,7 @@ paged_attention_few_kernel(RowsView<const float> q, PagesView<const float> kp, P
             const int at = w * R + r;
             const float m2 = jm[2 * at], l2 = jm[2 * at + 1], top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.0f : top * c2;
             const float ca = exp2_fast(fmaf(m[r], c2, -base)), cb = exp2_fast(fmaf(m2, c2, -base));
-            l[r] = l[r] * ca + l2 * cb;
+            l[r] = joined_sum(top, l[r], ca, l2, cb);
             m[r] = top;
 #pragma unroll
             for (int i = 0; i < COLS; ++i) o[r][i] = o[r][i] * ca + joint[at * D + lane * COLS + i] * cb;
@@ -835,7 +835,7 @@ paged_attention_few_kernel(RowsView<const float> q, PagesView<const float> kp, P
           const int64_t t = use.r.first + local[r];
           if (whole) {
             const bool seen = !(m[r] == -INFINITY && l[r] == 0.0f);
-            const float inv = seen ? 1.0f / l[r] : 0.0f;
+            const float inv = inverse_sum(m[r], l[r]);
             float* po = out.ptr + t * out.sn + h * out.sh + lane * COLS;
 #pragma unroll
             for (int i = 0; i < COLS; ++i) { const float x = o[r][i] * inv; wrong |= !isfinite(x); po[i] = x; }
@@ -881,6 +881,7 @@ paged_attention_join_kernel(RowsView<T> out, float* __restrict__ lse, TileWork w
     const int r = r0 + warp / shares;
     const bool live = r < u.rows;
     float top = -INFINITY, l = 0.0f;                                      // maxima in log2 units
+    bool minus = false;                                                   // a piece saw scores of -inf alone
     float4 o[COLS];                                                       // columns 4 lane .. 4 lane + 3, and 128 more for a head of 256
 #pragma unroll
     for (int i = 0; i < COLS; ++i) o[i] = make_float4(0, 0, 0, 0);
@@ -912,12 +913,14 @@ paged_attention_join_kernel(RowsView<T> out, float* __restrict__ lse, TileWork w
         if (p0 + k * shares >= u.pieces) break;
         const float w = exp2_fast(ml[k].x - base);
         l = fmaf(ml[k].y, w, l);
+        minus |= ml[k].y < 0.0f;
 #pragma unroll
         for (int i = 0; i < COLS; ++i) {
           o[i].x = fmaf(v[i][k].x, w, o[i].x); o[i].y = fmaf(v[i][k].y, w, o[i].y); o[i].z = fmaf(v[i][k].z, w, o[i].z); o[i].w = fmaf(v[i][k].w, w, o[i].w);
         }
       }
     }
+    l = only_minus_inf(minus, top, l);
     if (shares > 1) {                                                     // the same for all warps: a block-wide exchange
       if (lane == 0) { s_m[warp] = top; s_l[warp] = l; }
 #pragma unroll
@@ -932,6 +935,7 @@ paged_attention_join_kernel(RowsView<T> out, float* __restrict__ lse, TileWork w
         for (int w = 0; w < shares; ++w) {
           const float c = exp2_fast(s_m[warp + w] - base);
           l = fmaf(s_l[warp + w], c, l);
+          minus |= s_l[warp + w] < 0.0f;
 #pragma unroll
           for (int i = 0; i < COLS; ++i) {
             const int d = 4 * lane + 128 * i;
@@ -942,13 +946,14 @@ paged_attention_join_kernel(RowsView<T> out, float* __restrict__ lse, TileWork w
         }
       }
       __syncthreads();
+      l = only_minus_inf(minus, top, l);
     }
     if (live && part == 0) {
       const int g = u.row + r;
       const int64_t t = u.first + g / group;
       const int h = u.kv_head * group + g % group;
       const bool seen = !(top == -INFINITY && l == 0.0f);
-      const float inv = seen ? 1.0f / l : 0.0f;
+      const float inv = inverse_sum(top, l);
       T* po = out.ptr + t * out.sn + h * out.sh;
 #pragma unroll
       for (int i = 0; i < COLS; ++i) {

@@ -48,6 +48,12 @@ ojc_status paged_attention_tcgen05(const AttnCall& c, int tiles);
 #ifdef __CUDACC__
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+// A row's softmax so far is (maximum, sum). A row, or a piece of one, that saw scores of -inf alone has maximum -inf and this sum: among others it weighs
+// nothing, alone it is 0 / 0. Sum 0 under -inf is a row that saw nothing, NaN one that saw NaN.
+constexpr float ONLY_MINUS_INF = -1.0f;
+__device__ __forceinline__ float only_minus_inf(bool any, float m, float l) { return any && m == -INFINITY && l == 0.0f ? ONLY_MINUS_INF : l; }
+__device__ __forceinline__ float joined_sum(float top, float l, float c, float l2, float c2) { return top == -INFINITY ? l + l2 : l * c + l2 * c2; }
+__device__ __forceinline__ float inverse_sum(float m, float l) { return m != -INFINITY ? 1.0f / l : l == 0.0f ? 0.0f : NAN; }
 constexpr float LOG2_E = 1.4426950408889634f, LN_2 = 0.6931471805599453f;
 
 // The first place that a row of the request can see (positions of new tokens are at least `cached`). Pages that lie wholly before it are never looked up:

@@ -483,11 +483,11 @@ paged_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_k, const _
       if (unit_done || f + 1 == todo) {
         if (!mbar_wait(bar(C::PVFULL + g), f & 1, fault, abort_flag)) { ok = false; break; }
         fence_after();
-        if (any && !have) l = NAN;                                // every score -inf (or NaN): what the formula gives
+        if (!have) l = only_minus_inf(any, -INFINITY, l);
         const bool starts = f - piece == use.block, whole = unit_done && starts;
         const int n = use.row_tile * TILE_ROWS + g * ROWS + t, h = use.hk * args.group + (row.live ? n % args.group : 0);
         const int64_t token = use.r.first + row.local;
-        const float inv = any ? 1.0f / l : 0.0f;
+        const float inv = inverse_sum(have ? m : -INFINITY, l);
         bf16* dst = args.out.ptr + token * args.out.sn + h * args.out.sh;
         const int64_t at = (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * TILE_ROWS + g * ROWS + t;
         if (warp_live) {

@@ -210,3 +210,32 @@ def test_f32_operands_at_the_ends_of_the_range(be, h, hk, d, cached, new):
     c.v[first, off, :, 2], c.v[first, off, :, 3] = -0.5 * big, big              # at one place: the running sums are not normalised
     got, lse = c.check(be)
     assert np.all(np.isfinite(got))
+
+
+INFINITE = [(kind, h, hk, d, cached, new, page, tree) for kind, h, hk, d, new, page, tree in [
+    ("rows", 4, 2, 40, 3, 8, True), ("few f32", 4, 2, 64, 1, 16, False), ("few f32", 1, 1, 128, 3, 16, True), ("tiles f32", 8, 1, 96, 1, 16, True), ("tiles f32", 4, 1, 64, 9, 16, True),
+    ("tiles", 8, 1, 128, 1, 16, True), ("tiles", 4, 1, 64, 3, 16, True), ("tiles", 4, 1, 80, 7, 16, True), ("tcgen05", 2, 1, 64, 30, 16, True), ("tcgen05", 4, 1, 128, 40, 16, True)]
+    for cached in (16, 64, 5000)]
+
+
+@pytest.mark.parametrize("kind,h,hk,d,cached,new,page,tree", INFINITE)
+@pytest.mark.parametrize("where", ["a new token", "the first places", "all but one", "all"])
+def test_scores_of_minus_infinity_weigh_nothing(be, kind, h, hk, d, cached, new, page, tree, where):
+    """However the keys are shared out: places that score -inf alone in a warp or a piece, next to others, in all but one place, in all (then the formula's NaN)."""
+    from ojas_b200 import OjasError
+    bf16 = "f32" not in kind
+    c = Case(72 + d, [cached], [new], h, hk, d, page, tree, bf16)
+    c.q[..., 0] = 1.0
+    drop = {"a new token": [cached], "the first places": list(range(cached - 3)), "all but one": [p for p in range(cached + new) if p != 5], "all": list(range(cached + new))}[where]
+    want, want_lse, tol, lse_tol = scored_minus_infinity(c, drop)
+    q, out, lse = floats(be, c.q, bf16), floats(be, np.zeros(c.q.shape), bf16), be.zeros(c.q.shape[:2])
+    be.paged_attention_forward(q, floats(be, c.k, bf16), floats(be, c.v, bf16), u32(be, c.tables), u32(be, c.cached), u32(be, c.starts),
+                               masks=be.upload(c.masks) if c.masks is not None else None, positions=u32(be, c.positions), out=out, lse=lse)
+    if where == "all":
+        with pytest.raises(OjasError) as e:
+            be.sync()
+        assert e.value.kind == "NonFinite"
+        assert np.all(np.isnan(out.numpy())) and np.all(np.isnan(lse.numpy()))
+        return
+    be.sync()
+    assert np.all(np.abs(out.numpy() - want) <= tol) and np.all(np.abs(lse.numpy() - want_lse) <= lse_tol)
