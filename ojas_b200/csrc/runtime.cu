@@ -230,7 +230,7 @@ static ojc_status report_fault(ojc_backend* be, const char* op) {
   if (first == OP_ID_RANGE) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "a token id or target on the device is outside the vocabulary");
   if (first == OP_PAGED_RANGE) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "a page, slot, length or tree parent of the paged cache on the device is out of range");
   if (first == OP_PAGED_FULL) return ojc_fail(OJC_ERR_CAPACITY_EXCEEDED, op, "the free pages of the paged cache ran out on the device");
-  if (first == OP_GEMM_WAIT) return ojc_fail(OJC_ERR_WAIT_TIMEOUT, op, "a tensor-pipeline wait inside a GEMM kernel ran out");
+  if (first == OP_GEMM_WAIT) return ojc_fail(OJC_ERR_WAIT_TIMEOUT, op, "a tensor-pipeline wait inside a matrix-product or attention kernel ran out");
   return ojc_fail(OJC_ERR_NON_FINITE, ojc_op_name(first), std::string("non-finite value raised on the device, reported at ") + op);
 }
 

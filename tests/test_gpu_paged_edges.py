@@ -239,3 +239,16 @@ def test_scores_of_minus_infinity_weigh_nothing(be, kind, h, hk, d, cached, new,
         return
     be.sync()
     assert np.all(np.abs(out.numpy() - want) <= tol) and np.all(np.abs(lse.numpy() - want_lse) <= lse_tol)
+
+
+def test_an_expired_wait_is_not_laid_to_one_kind_of_kernel(be):
+    """The matrix products, the attention and the paged attention share the bounded wait and its word; the report names none of them alone."""
+    import ctypes as C
+    from ojas_b200 import OjasError
+    from ojas_b200._lib import lib
+    from ojas_b200.backend import _check
+    gave_up = C.c_int32(-1)
+    with pytest.raises(OjasError) as e:
+        _check(lib.ojc_selftest_bounded_wait(be._handle, C.c_uint64(2_000_000), C.byref(gave_up)))
+    assert e.value.kind == "WaitTimeout" and "matrix-product or attention" in str(e.value)
+    be.sync()
