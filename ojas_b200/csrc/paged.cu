@@ -506,7 +506,7 @@ ojc_status ojc_rope_plan(const ojc_rope_spec* spec, ojc_rope* rope) {
   if (s.layout != 0 && s.layout != 1) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "layout is 0 (half) or 1 (interleaved)");
   if (s.scaling < 0 || s.scaling > 3) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "scaling is 0 (none), 1 (linear), 2 (base) or 3 (by turns)");
   if (!(s.base >= 1.0) || !std::isfinite(s.base)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "base must be finite and at least 1");
-  if (!std::isfinite(s.amplitude)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "amplitude must be finite");
+  if (!std::isfinite((float)s.amplitude)) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "amplitude must be finite in F32");   // as the plan holds it
   if (s.scaling && (!(s.factor >= 1.0) || !std::isfinite(s.factor))) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "factor must be finite and at least 1");
   if (s.scaling == 2 && s.rotary_dim == 2) return ojc_fail(OJC_ERR_OUT_OF_RANGE, op, "base scaling needs more than one pair");
   if (s.scaling == 3 && (!(s.original_length > 0.0) || !std::isfinite(s.original_length) || !std::isfinite(s.low_turns) || !std::isfinite(s.high_turns) || !(s.high_turns > s.low_turns)))

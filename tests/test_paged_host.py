@@ -204,3 +204,11 @@ def test_paged_plan_held_refusals(handle):
     with pytest.raises(OjasError) as e:
         be.paged_plan(*[t((3,), u32)] * 4, t((3, 4), u32), 16, tokens=4, starts=t((4,), u32), slots=t((4,), u32), positions=t((4,), u32), free_head_out=t((1,), u32), held_pages_out=good)
     assert e.value.kind == "Shape"
+
+
+def test_an_amplitude_that_f32_does_not_hold_is_refused():
+    assert CudaBackend.rope_plan(RopeSpec(8, amplitude=3.4e38)).amplitude == np.float32(3.4e38)
+    for amplitude in (1e39, -1e39, 1e300):
+        with pytest.raises(OjasError) as e:
+            CudaBackend.rope_plan(RopeSpec(8, amplitude=amplitude))
+        assert e.value.kind == "OutOfRange"
