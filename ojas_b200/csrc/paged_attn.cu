@@ -1049,12 +1049,16 @@ template <class T, int D>
 ojc_status tiles_by_rows(const AttnCall& c) {
   // rows of a KV head in a request of average length: what the host knows without a readback
   const int64_t rows = (c.a.tokens + c.ix.batch - 1) / c.ix.batch * (c.a.heads / c.a.kv_heads);
-  // More than 32 rows: tcgen05 (48 drafts over 4000 cached, 16 heads of 128: 55 us against 76; 100 drafts 61 against 117). 17 to 32 rows: its tiles of 128 rows
-  // are mostly empty and the tiles here are ahead (31 drafts: 51 against 57 us at 1000 cached, 60 against 62 at 4000), except over long contexts, where the
-  // page copies by boxes count (20 rows over 131 thousand: 107 against 123 us).
+  // More than 32 rows: tcgen05 (48 drafts over 4000 cached, 16 heads of 128: 55 us against 76; 100 drafts 61 against 117).
+  // 17 to 32 rows, tiles here against tcgen05 in us, 31 drafts of 16 heads of 128: one request of 300, 4095 and 65536 cached 18/15, 40/28 and 135/107; 16 requests
+  // 35/37, 99/103 and, of 16384, 291/249; 64 requests of 300 84/120, of 4095 316/320 (4 tokens of 32/4 heads: 64 of 300 31/38, of 16384 288/248). So tcgen05
+  // while units do not queue behind one another, each paying for a tile of 128 rows that is mostly empty, and else where the tables are made for long
+  // requests (how long they are is not known here). At 64 columns its copies are half as large and its empty rows count for more: one request of 131
+  // thousand, 5 drafts of 32/8 heads, 85/102; 8 of 4095, 31 drafts, 46/60. (Ahead only for a single request of up to 16384: 36/32.)
   // Heads that leave columns of the operands empty, 63 rows: 68 us here against 63 at 96 columns and 4000 cached, 77 against 83 at 300 cached, 43 against 56 at
   // 32 columns; from 65 rows on a unit here is two row tiles (255 rows: 573 us against 208 at 96 columns, 282 against 180 at 32).
-  const bool whole = D == 64 || D == 128, wide = whole ? rows > 32 || (rows > 16 && c.ix.width * c.ix.page >= 32768) : rows > 64;
+  const bool few_units = c.ix.batch * c.a.kv_heads <= REDUCE_SMS, long_tables = c.ix.width * c.ix.page >= 32768;
+  const bool wide = D == 128 ? rows > 32 || (rows > 16 && (few_units || long_tables)) : rows > (D == 64 ? 32 : 64);
   if (D <= 128 && wide && paged_attention_tcgen05_takes(c)) return paged_attention_tcgen05(c, rows > 128 ? 2 : 1);
   if constexpr (std::is_same<T, float>::value && D % 32 == 0) {
     if (rows == 1) return few_launch<D, 1>(c);

@@ -252,3 +252,16 @@ def test_an_expired_wait_is_not_laid_to_one_kind_of_kernel(be):
         _check(lib.ojc_selftest_bounded_wait(be._handle, C.c_uint64(2_000_000), C.byref(gave_up)))
     assert e.value.kind == "WaitTimeout" and "matrix-product or attention" in str(e.value)
     be.sync()
+
+
+@pytest.mark.parametrize("h,hk,d,new", [(4, 4, 64, 20), (8, 2, 64, 5), (16, 16, 128, 17), (8, 2, 128, 8)])
+@pytest.mark.parametrize("requests", [1, 20])
+def test_seventeen_to_thirty_two_rows_in_narrow_and_wide_tables(be, h, hk, d, new, requests):
+    """Either kernel for these rows, by the number of units and (128 columns) the tables' width; at 64 columns the width has no say, so the bits are the same."""
+    rng = np.random.default_rng(80)
+    c = Case(81, [int(x) for x in rng.integers(1, 400, requests)], [new] * requests, h, hk, d, 16, True, True, pad=1)
+    out, lse = c.check(be)
+    c.tables = np.concatenate([c.tables, np.full((requests, 2100), 0x7FFFFFFF, np.int64)], 1)
+    wide = c.check(be)
+    if d == 64 or requests * hk <= 148:
+        assert np.array_equal(wide[0], out) and np.array_equal(wide[1], lse)
