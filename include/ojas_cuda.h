@@ -240,16 +240,22 @@ ojc_status ojc_rope_backward(ojc_backend* be, const ojc_rope* rope, const ojc_te
  * contiguous). With rope (and positions [N]) k is rotated on the way. A row with slot OJC_NONE is skipped; the other slots of a call are distinct. */
 ojc_status ojc_paged_kv_write(ojc_backend* be, ojc_tensor* k_pages, ojc_tensor* v_pages, const ojc_tensor* k, const ojc_tensor* v, const ojc_tensor* slots, const ojc_rope* rope,
                               const ojc_tensor* positions);
-/* q, out [N, H, D] against the pages (all F32, or all BF16 with f32 sums), through their strides (D contiguous, at most 256); lse [N, H] F32 (optional).
+/* q, out [N, H, D] against the pages (all F32 or all BF16), through their strides (D contiguous, at most 256); lse [N, H] F32 (optional).
  * Head h reads KV head h / (H / Hkv), the scale is 1 / sqrt(D). Token i of request b sees the cached places below cached_lens[b] and, of the
  * request's new tokens, those whose bits are set in row i of masks [N, words], or without masks those up to itself; of all these, with window >= 1,
  * only those whose position is above its own minus window (the position of a cached place is the place, that of a new token its entry of positions
  * [N], at least the cached length; without positions cached length + i). The new tokens' keys and values are in the cache already (paged_kv_write). What
  * masked places hold is never looked at: NaN or infinity there does no harm. Entries of block_tables for pages wholly before place cached_lens[b] -
- * window + 1 are not read, so such pages may have been released; from there to the request's last token every entry has to name a page. A row that sees nothing is 0 with lse -inf. Rows from starts[B] on are left as they are. A
- * non-finite value that a row does see surfaces as NonFinite. A call with 2^31 - 1 blocks of 64 or 128 keys or more, over all row tiles and KV heads,
- * computes nothing and surfaces as OutOfRange. workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or
- * NULL for the library's own (refused while the stream is being captured). */
+ * window + 1 are not read, so such pages may have been released; from there to the request's last token every entry has to name a page. A row that
+ * sees nothing is 0 with lse -inf. A place that scores -inf weighs nothing; a row all of whose places do is NaN. A result that is not finite surfaces as
+ * NonFinite. Rows from starts[B] on are left as they are. A call with 2^31 - 1 blocks of 64 or 128 keys or more, over all row tiles and KV heads,
+ * computes nothing and surfaces as OutOfRange.
+ * Scores, maxima, sums and outputs are held in F32. With BF16 operands the weights exp(s - max) are rounded to BF16 for their product with the values
+ * (the sum takes them unrounded), as in the SDPA family's BF16 tier: each output is off by at most 2^-8 of the weighted mean of the values' magnitudes,
+ * beside its own rounding. With F32 operands and more than four rows to a KV head the products drop 2^-22 (scores) and 2^-21 (outputs) of their size.
+ * Which kernel runs, and with it the rounding of the last bits, goes by types, head_dim, alignment, table width and N / B (so by the capacity N, not by
+ * the tokens in it). workspace: device memory of ojc_paged_attention_workspace_bytes for these q and pages, or NULL for the library's own (refused while
+ * the stream is being captured). */
 ojc_status ojc_paged_attention_workspace_bytes(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, uint64_t* bytes);
 ojc_status ojc_paged_attention_forward(ojc_backend* be, const ojc_tensor* q, const ojc_tensor* k_pages, const ojc_tensor* v_pages, const ojc_tensor* block_tables, const ojc_tensor* cached_lens,
                                        const ojc_tensor* starts, const ojc_tensor* masks, const ojc_tensor* positions, int64_t window, ojc_tensor* out, ojc_tensor* lse, void* workspace,

@@ -112,7 +112,9 @@ paged_attention_rows_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVie
 // copies through the block table (a warp's lanes look up their keys' pages one block ahead of the copies). With one row tile (MW 1) the four warps share
 // out the keys of a block and each waits for its own rows only; with MW 2 and 4 they share out rows, so that a key is used by 16 * MW rows once loaded.
 // Products: mma.sync m16n8k16 (BF16), or m16n8k8 TF32 with each F32 operand split in two (hi*hi + hi*lo + lo*hi: what is
-// dropped is 2^-22 of a product, 2^-21 of a weight times a value).
+// dropped is 2^-22 of a product, 2^-21 of a weight times a value). Weights are rounded to BF16 for the BF16 product, as the operand has to be; the running
+// sum takes them unrounded. Against 64 bits: rms error 1.7e-4 of outputs of rms 0.096 for 64 single tokens over up to 8191 places, 3.0e-4 of 0.13 for trees
+// of 63, where F32 weights have 1.6e-4 and 2.1e-4 (the output's own rounding).
 constexpr int TILE_WARPS = 4;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -33,7 +33,7 @@ struct AttnCall {
   const ojc_tensor *q, *k, *v; ojc_tensor* out; float* lse;
   PassIndex ix; AttnDims a; float scale; TileWork work;
 };
-// CTAs to launch: one wave, or fewer where the longest requests that the tables allow would not give each the two blocks that a share has at least
+// CTAs to launch: one wave, or fewer where the longest requests that the tables allow have no block for each
 inline unsigned attn_ctas(const AttnCall& c, int wave, int tile_rows, int keys) {
   const int64_t rows = c.a.tokens * (c.a.heads / c.a.kv_heads), tiles = (rows + tile_rows - 1) / tile_rows + c.ix.batch;
   const double most = (double)tiles * (double)c.a.kv_heads * (double)(c.ix.width * c.ix.page / keys + 1);
