@@ -196,7 +196,8 @@ paged_attention_tiles_kernel(RowsView<const T> q, PagesView<const T> kp, PagesVi
   Cursor<BLOCK_KEYS> ahead = use;                                                                                   // the block whose pages are looked up next
 
   // ---- copies: warp w fetches WARP_KEYS keys of a block from number w * WARP_KEYS on; with 16, lane l looks up key l's row of K and lane 16 + l its row of V,
-  // with 32 a lane does both. Places behind the last one repeat it, those before the first that a row can see repeat that one: what lies there is masked like any place that is not seen.
+  // with 32 a lane does both. Places behind the last one repeat it, those before the first that a row can see repeat that one: what lies there is masked
+  // like any place that is not seen.
   const PagesView<const T>& mine = lane < 16 ? kp : vp;
   const char* const mine_ptr = (const char*)mine.ptr;
   const int64_t mine_sp = mine.sp * (int)sizeof(T), mine_st = mine.st * (int)sizeof(T), mine_sh = mine.sh * (int)sizeof(T);

@@ -265,3 +265,32 @@ def test_seventeen_to_thirty_two_rows_in_narrow_and_wide_tables(be, h, hk, d, ne
     wide = c.check(be)
     if d == 64 or requests * hk <= 148:
         assert np.array_equal(wide[0], out) and np.array_equal(wide[1], lse)
+
+
+def test_held_pages_with_the_largest_batch_and_many_tokens(be):
+    """More lengths than the default shared memory holds, four tokens to a thread; every other request already holds a page more than its cached places need."""
+    batch, page = 24000, 16
+    cached, new = [int(x) for x in np.arange(batch) % 37], [int(x) for x in (np.arange(batch) * 7) % 19]
+    held = [-(-c // page) + (b & 1) for b, c in enumerate(cached)]
+    tables, free = np.arange(batch * 5).reshape(batch, 5), np.arange(batch * 5, batch * 8)[::-1].copy()
+    want, head, held_after, entered = held_plan(cached, new, held, free, 2, tables, page)
+    d_tables = u32(be, tables)
+    got = be.paged_plan(u32(be, cached), u32(be, new), u32(be, free), u32(be, [2]), d_tables, page, tokens=sum(new) + 3, held_pages=u32(be, held))
+    be.sync()
+    assert np.array_equal(got.slots.numpy(), np.array(want + [NONE] * 3, np.uint32)) and list(got.held_pages.numpy()) == held_after and got.free_head.numpy()[0] == head
+    assert np.array_equal(d_tables.numpy(), entered)
+
+
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("h,hk,d,bf16", [(2, 1, 64, True), (2, 2, 128, True), (1, 1, 64, False)])
+def test_a_long_piece_of_a_prompt(be, window, h, hk, d, bf16):
+    Case(82, [0, 190], [1300, 1030], h, hk, d, 64, False, bf16).check(be, window=window)
+
+
+@pytest.mark.parametrize("window", [None, 64])
+@pytest.mark.parametrize("h,hk,d,bf16", [(2, 2, 64, True), (4, 1, 128, True), (2, 2, 64, False)])
+def test_a_piece_of_a_prompt_among_single_tokens(be, window, h, hk, d, bf16):
+    cached = [int(x) for x in np.random.default_rng(83).integers(0, 300, 64)]
+    new = [1] * 64
+    new[40] = 512
+    Case(83, cached, new, h, hk, d, 16, False, bf16, pad=5).check(be, window=window)
